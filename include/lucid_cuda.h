@@ -298,6 +298,71 @@ int32_t lc_dynamic_linear_f32(const float* x, int64_t ldx, int64_t M, int64_t K,
                               const int32_t* wsum, void* out, int32_t out_dtype, int64_t ldo, void* workspace,
                               int64_t workspace_bytes, int32_t workspace_is_fresh, int32_t* status, void* stream);
 
+/* ---- int8 Linear with a fused epilogue, one or many groups -------------
+ * The dynamically quantized Linear (lucid/nn/quantized/dynamic/linear.py:85-92) with what a transformer
+ * block puts behind it, and the same product grouped by expert (the reference has neither):
+ *   out[m,n] = act(f32(acc - zx*wsum[e,n]) * sx[m] * sw[e,n] + bias[e,n]) + residual[m,n],
+ *   acc      = sum_k q[m,k] * wq[e,n,k]  (int32, exact),  e = the group whose rows contain m.
+ * q [rows, ldq]: int8 (or uint8, q_unsigned) codes, rows sorted by group; offsets [groups + 1] on the device:
+ * group e owns rows offsets[e] .. offsets[e+1] (ascending; values are clamped to [0, rows]).  offsets NULL:
+ * one group of all rows, the dense Linear.  Rows behind the last group's come out as zeros.
+ * wq [groups, N, ldw] with group_stride elements between groups; sw / bias / wsum [groups, N]; sx one value or
+ * one per row (sx_per_row); zx a device scalar, together with wsum, or both NULL.
+ * activation: LC_ACT_*; with LC_ACT_SWIGLU the N weight rows are blocks of 8 gate rows and the matching 8 up
+ * rows, and out and residual have N/2 columns: silu(gate) * up.  residual: of out_dtype, or NULL.
+ * out_dtype LC_F32, LC_BF16 or LC_F16.  Rows of q and wq on 16-byte boundaries, K <= 65536, groups <= 1024.
+ * variant: 0 automatic, 1 128 x 64 tiles with K split over a cluster, 2 256 x 256 tiles of CTA pairs, all with
+ * identical results; | LC_QLINEAR_WAIT_TEST as for lc_qlinear_i8_ex.  status: see lc_qlinear_check_status. */
+#define LC_ACT_NONE 0
+#define LC_ACT_RELU 1
+#define LC_ACT_GELU 2      /* 0.5 v (1 + erf(v / sqrt 2)) */
+#define LC_ACT_GELU_TANH 3 /* 0.5 v (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3))) */
+#define LC_ACT_SILU 4
+#define LC_ACT_SWIGLU 5
+int32_t lc_grouped_qlinear_i8(const void* q, int32_t q_unsigned, int64_t ldq, int64_t rows,
+                              const int32_t* offsets, int64_t groups, const int8_t* wq, int64_t ldw,
+                              int64_t group_stride, int64_t N, int64_t K, const float* sx, int32_t sx_per_row,
+                              const float* zx, const int32_t* wsum, const float* sw, const float* bias,
+                              int32_t activation, const void* residual, int64_t ldr, void* out,
+                              int32_t out_dtype, int64_t ldo, int32_t* status, int32_t variant, void* stream);
+
+/* Row-wise symmetric int8 quantization of fp32, bf16 or f16 rows:
+ *   s = max(max|x| / 127.5, 1e-8), code = clamp(rint(x * (1/s)), -128, 127)   (IEEE fp32 per step, NaN -> 0).
+ * positions [rows, copies] (or NULL): row t's codes and scale go to rows positions[t, 0 .. copies) of codes /
+ * scale (entries outside [0, out_rows) are skipped); NULL: to row t.  valid: device count of rows of x to
+ * quantize, or NULL for all. */
+int32_t lc_quantize_tokens(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ldx,
+                           const int32_t* positions, int64_t copies, int64_t out_rows, const int32_t* valid,
+                           int8_t* codes, int64_t ldq, float* scale, void* stream);
+
+/* lc_quantize_tokens followed by lc_grouped_qlinear_i8 on the same stream, codes and scales in `workspace`
+ * (lc_expert_linear_workspace_bytes(rows, K), 256-byte aligned, free again when the call's work is done).
+ * positions [x_rows, top_k] with rows = x_rows * top_k: token t feeds the rows positions[t, :]; NULL: x holds
+ * the rows in group order already (x_rows = rows).  Dense Linear: positions and offsets NULL, groups 1. */
+int64_t lc_expert_linear_workspace_bytes(int64_t rows, int64_t K);
+int32_t lc_expert_linear(const void* x, int32_t x_dtype, int64_t x_rows, int64_t ldx, const int32_t* positions,
+                         int64_t top_k, const int32_t* offsets, int64_t groups, int64_t rows, const int8_t* wq,
+                         int64_t ldw, int64_t group_stride, int64_t N, int64_t K, const float* sw,
+                         const float* bias, int32_t activation, const void* residual, int64_t ldr, void* out,
+                         int32_t out_dtype, int64_t ldo, void* workspace, int64_t workspace_bytes,
+                         int32_t* status, void* stream);
+
+/* Router: for each token the top_k largest of its logits [tokens, ld] (equal logits: lowest expert first),
+ * weights = softmax over all experts (renormalize: over the chosen ones), and every choice's row in the order
+ * "by expert, then by token": offsets [experts + 1], positions / chosen / weights [tokens, top_k].  Logits of
+ * -inf and NaN are never chosen and carry no weight: chosen and positions are -1 and weights 0 where a token
+ * has fewer than top_k others.  experts <= 1024, top_k <= 32.  workspace: lc_route_experts_workspace_bytes. */
+int64_t lc_route_experts_workspace_bytes(int64_t tokens, int64_t experts);
+int32_t lc_route_experts(const void* logits, int32_t dtype, int64_t tokens, int64_t experts, int64_t ld,
+                         int64_t top_k, int32_t renormalize, float* weights, int32_t* chosen, int32_t* offsets,
+                         int32_t* positions, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* out[t,:] = sum_j weights[t,j] * y[positions[t,j],:] + residual[t,:], added in the order of j in fp32 and
+ * rounded once; positions outside [0, rows) contribute nothing.  y, residual and out share one dtype. */
+int32_t lc_combine_experts(const void* y, int32_t dtype, int64_t rows, int64_t cols, int64_t ldy,
+                           const float* weights, const int32_t* positions, int64_t tokens, int64_t top_k,
+                           const void* residual, int64_t ldr, void* out, int64_t ldo, void* stream);
+
 /* row sums of an int8 matrix as int32 (the zero-point correction term) */
 int32_t lc_rowsum_s8(const int8_t* b, int64_t rows, int64_t cols, int64_t ldb, int32_t* out,
                      void* stream);

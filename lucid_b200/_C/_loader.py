@@ -70,6 +70,15 @@ SIGNATURES = {
     "lc_dynamic_linear_workspace_bytes": (_i64, [_i64, _i64]),
     "lc_dynamic_linear_f32": (_i32, [_p, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _f, _p, _i64, _i64, _p, _p, _p, _p, _i32,
                                      _i64, _p, _i64, _i32, _p, _p]),
+    "lc_grouped_qlinear_i8": (_i32, [_p, _i32, _i64, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _i32, _p, _p, _p, _p, _i32,
+                                     _p, _i64, _p, _i32, _i64, _p, _i32, _p]),
+    "lc_quantize_tokens": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _p, _p]),
+    "lc_expert_linear_workspace_bytes": (_i64, [_i64, _i64]),
+    "lc_expert_linear": (_i32, [_p, _i32, _i64, _i64, _p, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _p, _p, _i32, _p,
+                                _i64, _p, _i32, _i64, _p, _i64, _p, _p]),
+    "lc_route_experts_workspace_bytes": (_i64, [_i64, _i64]),
+    "lc_route_experts": (_i32, [_p, _i32, _i64, _i64, _i64, _i64, _i32, _p, _p, _p, _p, _p, _i64, _p]),
+    "lc_combine_experts": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _p, _i64, _p]),
     "lc_rowsum_s8": (_i32, [_p, _i64, _i64, _i64, _p, _p]),
     "lc_wo_gemm_16": (_i32, [_p, _i32, _i32, _i64, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _i32, _p, _p, _i32, _i32,
                              _p, _i32, _i64, _p, _i32, _p]),
@@ -100,10 +109,11 @@ for _name, (_res, _args) in SIGNATURES.items():
     _fn.argtypes = _args
 
 
-# The four entry points a decode-time forward calls once per layer, behind a CPython module that spares
+# The entry points a decode-time forward calls once per layer, behind a CPython module that spares
 # ctypes' marshalling (about 3 us per call with twenty arguments); ctypes serves them when the module has
 # not been built.  Same arguments, same status code.
-FAST_ENTRY_POINTS = ("lc_dynamic_linear_f32", "lc_group_matmul_ex", "lc_wo_linear_s8_ex", "lc_wo_swiglu_s8_ex")
+FAST_ENTRY_POINTS = ("lc_dynamic_linear_f32", "lc_group_matmul_ex", "lc_wo_linear_s8_ex", "lc_wo_swiglu_s8_ex",
+                     "lc_expert_linear", "lc_route_experts", "lc_combine_experts")
 try:
     from . import _fastcall as fast
 except ImportError:

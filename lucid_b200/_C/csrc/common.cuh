@@ -23,6 +23,10 @@ int sm_count();  // SM count of the current device (cached per device)
 int32_t encode_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner,
                              uint64_t rows, uint64_t stride_bytes, uint32_t box_inner, uint32_t box_rows,
                              CUtensorMapSwizzle swizzle);
+// the same with a third dimension of `planes` (one box covers one plane)
+int32_t encode_tensor_map_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner,
+                             uint64_t rows, uint64_t planes, uint64_t row_bytes, uint64_t plane_bytes,
+                             uint32_t box_inner, uint32_t box_rows, CUtensorMapSwizzle swizzle);
 
 // GEMV-shaped int8 x int8 product for up to 32 rows against a weight of 4 MB and more (qgemv_kernels.cu): same
 // arguments and bit-identical results as the tensor-core GEMM behind lc_qlinear_i8

@@ -1,0 +1,594 @@
+// The kernels around the experts' products: the router (top-k, softmax weights, rows sorted by expert), the
+// row-wise quantizer that also places each token's codes in expert order, and the weighted sum that brings
+// the experts' results back to their tokens.
+#include <mutex>
+
+#include "common.cuh"
+
+namespace lc {
+namespace {
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v);
+template <>
+__device__ __forceinline__ float to_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+// 16 bytes as floats
+template <typename T>
+struct Vec16 {
+  static constexpr int kN = 16 / sizeof(T);
+  T v[kN];
+  __device__ __forceinline__ void load(const T* p) { *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void load_stream(const T* p) {
+    *reinterpret_cast<uint4*>(v) = __ldcs(reinterpret_cast<const uint4*>(p));
+  }
+};
+
+// =============================================================================================
+// Router.  For each token: the top_k largest logits (equal logits: lowest expert first), their softmax
+// weights, and each choice's place in the order "by expert, then by token".
+//
+// A logit of -inf or NaN is never chosen and carries no weight (masked experts, padded tokens); what is not
+// chosen has expert -1, position -1 and weight 0.  +inf shares the weight with the other +inf of its row.
+//
+// One warp per token: the row sits in registers (EPL values per lane), each of the top_k rounds is a local
+// maximum and two warp-wide integer reductions (order-preserving bits of the value, then the lowest index).
+// A warp walks a contiguous run of tokens and counts its choices per expert in shared memory; a choice's
+// count is its rank inside the run.  Small batches (one CTA) finish in the same kernel; otherwise each CTA
+// leaves its counts and its ranks, and the second kernel adds what precedes them.  Every sum is an integer
+// one over a fixed order, so the result does not depend on scheduling.
+// =============================================================================================
+constexpr int kRouteMaxExperts = 1024;
+constexpr int kRouteMaxTopK = 32;
+
+// unsigned order = float order; NaN and -inf map to 0 (never chosen), -0 and +0 are equal
+__device__ __forceinline__ uint32_t order_bits(float v) {
+  if (!(v > -INFINITY)) return 0u;
+  const uint32_t b = __float_as_uint(v + 0.0f);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float order_value(uint32_t b) {
+  return __uint_as_float((b & 0x80000000u) ? (b & 0x7fffffffu) : ~b);
+}
+
+struct RouteParams {
+  const void* logits;
+  int64_t tokens, ld;
+  int experts, top_k, renormalize;
+  float* weights;      // [tokens, top_k]
+  int32_t* chosen;     // [tokens, top_k]
+  int32_t* positions;  // [tokens, top_k]
+  int32_t* offsets;    // [experts + 1]
+  int32_t* counts;     // [CTAs, experts], several CTAs only
+  int run;             // tokens per warp
+};
+
+// inclusive sum over the block of one int per thread; `tmp` holds 32 ints
+__device__ __forceinline__ int block_scan(int v, int* tmp) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  __syncthreads();
+  if (lane == 31) tmp[warp] = v;
+  __syncthreads();
+  if (warp == 0) {
+    int w = lane < warps ? tmp[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += u;
+    }
+    tmp[lane] = w;
+  }
+  __syncthreads();
+  return v + (warp ? tmp[warp - 1] : 0);
+}
+
+template <typename T, int EPL, bool ONE_CTA>
+__global__ void __launch_bounds__(ONE_CTA ? 1024 : 256) route_kernel(const RouteParams p) {
+  extern __shared__ int s_counts[];  // [warps][experts]; one CTA: then [experts] bases
+  __shared__ int s_tmp[32];
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int E = p.experts, K = p.top_k;
+  int* mine = s_counts + warp * E;
+  for (int i = threadIdx.x; i < warps * E; i += blockDim.x) s_counts[i] = 0;
+  pdl_launch_dependents();
+  pdl_wait();
+  __syncthreads();
+
+  const int64_t first = (static_cast<int64_t>(blockIdx.x) * warps + warp) * p.run;
+  const int64_t last = first + p.run < p.tokens ? first + p.run : p.tokens;
+  for (int64_t t = first; t < last; ++t) {
+    const T* row = static_cast<const T*>(p.logits) + t * p.ld;
+    uint32_t key[EPL];
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      const int e = i * 32 + lane;
+      key[i] = e < E ? order_bits(to_float<T>(row[e])) : 0u;
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) top = max(top, key[i]);
+    top = __reduce_max_sync(0xffffffffu, top);
+    const float largest = order_value(top);
+    // exp(v - largest); with an infinite largest value 1 for those equal to it and 0 for the rest
+    const bool finite = largest < INFINITY;
+    float total = 0.0f;
+    if (!p.renormalize && top) {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i)
+        if (key[i]) total += finite ? expf(order_value(key[i]) - largest) : (key[i] == top ? 1.0f : 0.0f);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
+    // lane j keeps the j-th choice
+    float my_p = 0.0f;
+    int my_e = -1;
+    uint32_t best = top;
+    for (int j = 0; j < K && best; ++j) {
+      uint32_t at = 0xffffffffu;
+#pragma unroll
+      for (int i = EPL - 1; i >= 0; --i)
+        if (key[i] == best) at = i * 32 + lane;
+      at = __reduce_min_sync(0xffffffffu, at);
+      const float pr = finite ? expf(order_value(best) - largest) : (best == top ? 1.0f : 0.0f);
+      if (p.renormalize) total += pr;
+      if (lane == j) {
+        my_p = pr;
+        my_e = static_cast<int>(at);
+      }
+      uint32_t next = 0;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) {
+        if (i * 32 + lane == static_cast<int>(at)) key[i] = 0u;
+        next = max(next, key[i]);
+      }
+      best = __reduce_max_sync(0xffffffffu, next);
+    }
+    if (lane < K) {
+      int rank = -1;
+      if (my_e >= 0) rank = mine[my_e]++;  // a token's choices are distinct experts: no two lanes meet
+      p.weights[t * K + lane] = my_e >= 0 ? __fdiv_rn(my_p, total) : 0.0f;
+      p.chosen[t * K + lane] = my_e;
+      p.positions[t * K + lane] = rank;  // rank inside this warp's run; completed below or by the second kernel
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+
+  // counts of the CTA, and each warp's start inside them
+  int* base = s_counts + warps * E;
+  for (int e0 = 0; e0 < E; e0 += blockDim.x) {
+    const int e = e0 + threadIdx.x;
+    int sum = 0;
+    if (e < E) {
+      for (int w = 0; w < warps; ++w) {
+        const int c = s_counts[w * E + e];
+        s_counts[w * E + e] = sum;
+        sum += c;
+      }
+      if (!ONE_CTA) p.counts[static_cast<int64_t>(blockIdx.x) * E + e] = sum;
+    }
+    if (ONE_CTA) {  // (1024 threads: one round covers all experts)
+      const int end = block_scan(sum, s_tmp);
+      if (e < E) {
+        base[e] = end - sum;
+        p.offsets[e + 1] = end;
+        if (e == 0) p.offsets[0] = 0;
+      }
+    }
+  }
+  __syncthreads();
+  for (int64_t i = first * K + lane; i < last * K; i += 32) {
+    const int e = p.chosen[i];
+    if (e >= 0) p.positions[i] += mine[e] + (ONE_CTA ? base[e] : 0);
+  }
+}
+
+// second kernel of a large batch: CTA b adds to its tokens' ranks the rows of the experts before and the
+// counts of the CTAs before it
+__global__ void __launch_bounds__(256) route_place_kernel(const RouteParams p, int ctas, int64_t tokens_per_cta) {
+  __shared__ int s_base[kRouteMaxExperts];
+  __shared__ int s_tmp[32];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int E = p.experts;
+  int carry = 0;
+  for (int e0 = 0; e0 < E; e0 += 256) {
+    const int e = e0 + threadIdx.x;
+    int before = 0, sum = 0;
+    if (e < E) {
+      const int32_t* c = p.counts + e;
+#pragma unroll 8
+      for (int b = 0; b < ctas; ++b) {
+        const int v = __ldg(c + static_cast<int64_t>(b) * E);
+        if (b < static_cast<int>(blockIdx.x)) before += v;
+        sum += v;
+      }
+    }
+    const int end = block_scan(sum, s_tmp);
+    if (e < E) {
+      s_base[e] = carry + end - sum + before;
+      if (blockIdx.x == 0) {
+        p.offsets[e + 1] = carry + end;
+        if (e == 0) p.offsets[0] = 0;
+      }
+    }
+    carry += s_tmp[7];
+  }
+  __syncthreads();
+  const int64_t first = blockIdx.x * tokens_per_cta;
+  const int64_t last = first + tokens_per_cta < p.tokens ? first + tokens_per_cta : p.tokens;
+  for (int64_t i = first * p.top_k + threadIdx.x; i < last * p.top_k; i += 256) {
+    const int e = p.chosen[i];
+    if (e >= 0) p.positions[i] += s_base[e];
+  }
+}
+
+constexpr int64_t kRouteOneCta = 128;  // tokens
+constexpr int kRouteRun = 16;          // tokens per warp of a large batch
+constexpr int64_t kRouteWarps = 8;
+
+template <typename T, int EPL>
+cudaError_t launch_route(RouteParams p, cudaStream_t st) {
+  if (p.tokens <= kRouteOneCta) {
+    p.run = static_cast<int>((p.tokens + 31) / 32);
+    const size_t smem = static_cast<size_t>(33) * p.experts * 4;
+    static std::once_flag flags[64];
+    static cudaError_t results[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    std::call_once(flags[dev], [dev]() {
+      results[dev] = cudaFuncSetAttribute(route_kernel<T, EPL, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          33 * EPL * 32 * 4);
+    });
+    if (results[dev] != cudaSuccess) return results[dev];
+    return launch_overlapped(route_kernel<T, EPL, true>, dim3(1), dim3(1024), smem, st, p);
+  }
+  p.run = kRouteRun;
+  const int64_t per_cta = kRouteWarps * p.run;
+  const int ctas = static_cast<int>((p.tokens + per_cta - 1) / per_cta);
+  cudaError_t err = launch_overlapped(route_kernel<T, EPL, false>, dim3(ctas), dim3(256),
+                                      static_cast<size_t>(kRouteWarps) * p.experts * 4, st, p);
+  if (err != cudaSuccess) return err;
+  return launch_overlapped(route_place_kernel, dim3(ctas), dim3(256), 0, st, p, ctas, per_cta);
+}
+
+template <typename T>
+cudaError_t dispatch_route(const RouteParams& p, cudaStream_t st) {
+  if (p.experts <= 32) return launch_route<T, 1>(p, st);
+  if (p.experts <= 64) return launch_route<T, 2>(p, st);
+  if (p.experts <= 128) return launch_route<T, 4>(p, st);
+  if (p.experts <= 256) return launch_route<T, 8>(p, st);
+  return launch_route<T, 32>(p, st);
+}
+
+// =============================================================================================
+// Row-wise symmetric int8 quantization of fp32 / bf16 / f16 rows:
+//   s = max(max|x| / 127.5, 1e-8), code = clamp(rint(x * (1/s)), -128, 127), NaN -> 0,
+// every step one IEEE fp32 operation (the per-row grid of lucid/nn/quantized/dynamic/linear.py's weights;
+// lucid/quantization/_qparams.py:186-205).  With `positions`, the codes and the scale of token t go to the
+// rows positions[t, 0..copies) (negative: nowhere); otherwise to row t.  `valid` (device): rows of x.
+//
+// The row stays in registers between the maximum and the codes, so x is read once.  The kernel lets its
+// successor start only after its own wait, so a successor may assume that whatever preceded this kernel is
+// complete.
+// =============================================================================================
+struct TokenParams {
+  const void* x;
+  int64_t rows, cols, ldx;
+  const int32_t* positions;
+  int copies;
+  int64_t out_rows;
+  const int32_t* valid;
+  int8_t* codes;
+  int64_t ldq;
+  float* scale;
+};
+
+__device__ __forceinline__ float token_scale(float largest) { return fmaxf(__fdiv_rn(largest, 127.5f), 1e-8f); }
+
+// TPR threads hold a row of up to TPR * ITEMS vectors; 256 / TPR rows (at least one) per CTA
+template <typename T, int TPR, int ITEMS>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) quantize_tokens_kernel(const TokenParams p) {
+  constexpr int VN = Vec16<T>::kN, THREADS = TPR < 256 ? 256 : TPR, ROWS = THREADS / TPR;
+  __shared__ float s_max[THREADS / 32];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int sub = threadIdx.x % TPR, warp = threadIdx.x >> 5;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / TPR;
+  const bool live = row < p.rows && (!p.valid || row < __ldg(p.valid));
+  const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+  const int vectors = static_cast<int>(p.cols / VN);
+  Vec16<T> v[ITEMS];
+  float largest = 0.0f;
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int at = i * TPR + sub;
+    if (live && at < vectors) v[i].load(x + static_cast<int64_t>(at) * VN);
+  }
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    if (live && i * TPR + sub < vectors) {
+#pragma unroll
+      for (int j = 0; j < VN; ++j) largest = fmaxf(largest, fabsf(to_float<T>(v[i].v[j])));  // (fmaxf drops NaN)
+    }
+  }
+  largest = warp_max(largest);
+  if (TPR > 32) {
+    if ((threadIdx.x & 31) == 0) s_max[warp] = largest;
+    __syncthreads();
+    constexpr int WPR = TPR / 32;
+    const int w0 = warp / WPR * WPR;
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) largest = fmaxf(largest, s_max[w0 + w]);
+  }
+  if (!live) return;
+  const float s = token_scale(largest), inv = __fdiv_rn(1.0f, s);
+  const int copies = p.positions ? p.copies : 1;
+  uint32_t packed[ITEMS][VN / 4];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+#pragma unroll
+    for (int j = 0; j < VN; j += 4)
+      packed[i][j / 4] = pack4_sat<false>(__fmul_rn(to_float<T>(v[i].v[j]), inv), __fmul_rn(to_float<T>(v[i].v[j + 1]), inv),
+                                          __fmul_rn(to_float<T>(v[i].v[j + 2]), inv),
+                                          __fmul_rn(to_float<T>(v[i].v[j + 3]), inv), 0.0f, false);
+  }
+  for (int c = 0; c < copies; ++c) {
+    const int64_t to = p.positions ? __ldg(p.positions + row * copies + c) : row;
+    if (to < 0 || to >= p.out_rows) continue;
+    if (sub == 0) p.scale[to] = s;
+    int8_t* q = p.codes + to * p.ldq;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int at = i * TPR + sub;
+      if (at < vectors) {
+        if (VN == 8)
+          *reinterpret_cast<uint2*>(q + static_cast<int64_t>(at) * VN) = make_uint2(packed[i][0], packed[i][VN / 4 - 1]);
+        else
+          *reinterpret_cast<uint32_t*>(q + static_cast<int64_t>(at) * VN) = packed[i][0];
+      }
+    }
+  }
+}
+
+// any length and alignment: one CTA per row, which is read twice (the second time from L1 / L2)
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_tokens_any_kernel(const TokenParams p) {
+  __shared__ float s_max[8];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t row = blockIdx.x;
+  if (p.valid && row >= __ldg(p.valid)) return;
+  const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+  float largest = 0.0f;
+  for (int64_t i = threadIdx.x; i < p.cols; i += 256) largest = fmaxf(largest, fabsf(to_float<T>(x[i])));
+  largest = warp_max(largest);
+  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = largest;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) largest = fmaxf(largest, s_max[w]);
+  const float s = token_scale(largest), inv = __fdiv_rn(1.0f, s);
+  const int copies = p.positions ? p.copies : 1;
+  for (int c = 0; c < copies; ++c) {
+    const int64_t to = p.positions ? __ldg(p.positions + row * copies + c) : row;
+    if (to < 0 || to >= p.out_rows) continue;
+    if (threadIdx.x == 0) p.scale[to] = s;
+    for (int64_t i = threadIdx.x; i < p.cols; i += 256)
+      p.codes[to * p.ldq + i] = static_cast<int8_t>(code_to_int(grid_code(to_float<T>(x[i]), inv, 0.0f), -128.0f, 127.0f));
+  }
+}
+
+template <typename T>
+cudaError_t launch_tokens(const TokenParams& p, cudaStream_t st) {
+  constexpr int VN = Vec16<T>::kN;
+  const int64_t vectors = p.cols / VN;
+  const bool vec = p.cols % VN == 0 && (p.ldx * sizeof(T)) % 16 == 0 && p.ldq % 8 == 0 && aligned(p.x, 16) &&
+                   aligned(p.codes, 8);
+  auto grid = [&](int rows_per_cta) { return dim3(static_cast<unsigned>((p.rows + rows_per_cta - 1) / rows_per_cta)); };
+  if (!vec || vectors > 4096) return launch_overlapped(quantize_tokens_any_kernel<T>, grid(1), dim3(256), 0, st, p);
+  if (vectors <= 32) return launch_overlapped(quantize_tokens_kernel<T, 32, 1>, grid(8), dim3(256), 0, st, p);
+  if (vectors <= 128) return launch_overlapped(quantize_tokens_kernel<T, 32, 4>, grid(8), dim3(256), 0, st, p);
+  if (vectors <= 512) return launch_overlapped(quantize_tokens_kernel<T, 128, 4>, grid(2), dim3(256), 0, st, p);
+  if (vectors <= 2048) return launch_overlapped(quantize_tokens_kernel<T, 512, 4>, grid(1), dim3(512), 0, st, p);
+  return launch_overlapped(quantize_tokens_kernel<T, 512, 8>, grid(1), dim3(512), 0, st, p);
+}
+
+// =============================================================================================
+// out[t] = sum_j weights[t,j] * y[positions[t,j]] + residual[t], the terms added in the order of j in fp32,
+// rounded once.  Positions of -1 contribute nothing.  HBM-bound: a thread owns 16 bytes of a row and has the
+// loads of four experts in flight.
+// =============================================================================================
+struct CombineParams {
+  const void* y;
+  int64_t rows, cols, ldy, tokens;
+  int top_k;
+  const float* weights;
+  const int32_t* positions;
+  const void* residual;
+  int64_t ldr;
+  void* out;
+  int64_t ldo;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) combine_kernel(const CombineParams p, int vectors) {
+  constexpr int VN = Vec16<T>::kN;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t t = at / vectors;
+  if (t >= p.tokens) return;
+  const int64_t col = (at - t * vectors) * VN;
+  float acc[VN];
+#pragma unroll
+  for (int i = 0; i < VN; ++i) acc[i] = 0.0f;
+  Vec16<T> res;
+  if (p.residual) res.load_stream(static_cast<const T*>(p.residual) + t * p.ldr + col);
+  for (int j0 = 0; j0 < p.top_k; j0 += 4) {
+    Vec16<T> v[4];
+    float w[4];
+    int32_t from[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      from[j] = j0 + j < p.top_k ? __ldg(p.positions + t * p.top_k + j0 + j) : -1;
+      if (from[j] >= p.rows) from[j] = -1;
+      w[j] = from[j] >= 0 ? __ldg(p.weights + t * p.top_k + j0 + j) : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (from[j] >= 0) v[j].load_stream(static_cast<const T*>(p.y) + from[j] * p.ldy + col);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (from[j] >= 0) {
+#pragma unroll
+        for (int i = 0; i < VN; ++i) acc[i] = fmaf(w[j], to_float<T>(v[j].v[i]), acc[i]);
+      }
+    }
+  }
+  if (p.residual) {
+#pragma unroll
+    for (int i = 0; i < VN; ++i) acc[i] += to_float<T>(res.v[i]);
+  }
+  Vec16<T> o;
+#pragma unroll
+  for (int i = 0; i < VN; ++i) o.v[i] = from_float<T>(acc[i]);
+  *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + t * p.ldo + col) = *reinterpret_cast<const uint4*>(o.v);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) combine_any_kernel(const CombineParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t t = at / p.cols;
+  if (t >= p.tokens) return;
+  const int64_t col = at - t * p.cols;
+  float acc = 0.0f;
+  for (int j = 0; j < p.top_k; ++j) {
+    const int32_t from = __ldg(p.positions + t * p.top_k + j);
+    if (from >= 0 && from < p.rows)
+      acc = fmaf(__ldg(p.weights + t * p.top_k + j), to_float<T>(static_cast<const T*>(p.y)[from * p.ldy + col]), acc);
+  }
+  if (p.residual) acc += to_float<T>(static_cast<const T*>(p.residual)[t * p.ldr + col]);
+  static_cast<T*>(p.out)[t * p.ldo + col] = from_float<T>(acc);
+}
+
+template <typename T>
+cudaError_t launch_combine(const CombineParams& p, cudaStream_t st) {
+  constexpr int VN = Vec16<T>::kN;
+  auto row_ok = [](const void* base, int64_t ld) { return aligned(base, 16) && (ld * sizeof(T)) % 16 == 0; };
+  const bool vec = p.cols % VN == 0 && row_ok(p.y, p.ldy) && row_ok(p.out, p.ldo) &&
+                   (!p.residual || row_ok(p.residual, p.ldr));
+  const int64_t items = p.tokens * (vec ? p.cols / VN : p.cols);
+  const dim3 grid(static_cast<unsigned>((items + 255) / 256));
+  if (vec) return launch_overlapped(combine_kernel<T>, grid, dim3(256), 0, st, p, static_cast<int>(p.cols / VN));
+  return launch_overlapped(combine_any_kernel<T>, grid, dim3(256), 0, st, p);
+}
+
+int32_t finish_launch(const char* what, cudaError_t err) {
+  if (err != cudaSuccess) return fail(LC_ERR_CUDA, "%s: %s", what, cudaGetErrorString(err));
+  return check_launch(what);
+}
+
+}  // namespace
+}  // namespace lc
+
+using namespace lc;
+
+extern "C" int64_t lc_route_experts_workspace_bytes(int64_t tokens, int64_t experts) {
+  if (tokens <= kRouteOneCta || experts <= 0) return 0;
+  const int64_t per_cta = kRouteWarps * kRouteRun;
+  return (tokens + per_cta - 1) / per_cta * experts * 4;
+}
+
+extern "C" int32_t lc_route_experts(const void* logits, int32_t dtype, int64_t tokens, int64_t experts, int64_t ld,
+                                    int64_t top_k, int32_t renormalize, float* weights, int32_t* chosen,
+                                    int32_t* offsets, int32_t* positions, void* workspace, int64_t workspace_bytes,
+                                    void* stream) {
+  if (tokens < 0 || experts < 1 || top_k < 1 || top_k > experts || ld < experts)
+    return fail(LC_ERR_INVALID_ARG, "route_experts: bad shape (1 <= top_k <= experts is required)");
+  if (experts > kRouteMaxExperts || top_k > kRouteMaxTopK)
+    return fail(LC_ERR_UNSUPPORTED, "route_experts: at most %d experts and top_k %d", kRouteMaxExperts, kRouteMaxTopK);
+  if (tokens * top_k > 0x7fffffffLL - 512) return fail(LC_ERR_UNSUPPORTED, "route_experts: too many tokens");
+  if (dtype != LC_F32 && dtype != LC_BF16 && dtype != LC_F16)
+    return fail(LC_ERR_UNSUPPORTED, "route_experts: dtype %d not supported", dtype);
+  if (!offsets) return fail(LC_ERR_INVALID_ARG, "route_experts: null pointer");
+  if (tokens == 0) {  // no token, no row: all offsets are zero
+    if (cudaMemsetAsync(offsets, 0, static_cast<size_t>(experts + 1) * 4, as_stream(stream)) != cudaSuccess)
+      return fail(LC_ERR_CUDA, "route_experts: %s", cudaGetErrorString(cudaGetLastError()));
+    return LC_OK;
+  }
+  if (!logits || !weights || !chosen || !positions) return fail(LC_ERR_INVALID_ARG, "route_experts: null pointer");
+  const int64_t need = lc_route_experts_workspace_bytes(tokens, experts);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 4)))
+    return fail(LC_ERR_WORKSPACE, "route_experts: workspace of %lld bytes required", (long long)need);
+  RouteParams p = {};
+  p.logits = logits;
+  p.tokens = tokens;
+  p.ld = ld;
+  p.experts = static_cast<int>(experts);
+  p.top_k = static_cast<int>(top_k);
+  p.renormalize = renormalize;
+  p.weights = weights;
+  p.chosen = chosen;
+  p.positions = positions;
+  p.offsets = offsets;
+  p.counts = static_cast<int32_t*>(workspace);
+  cudaStream_t st = as_stream(stream);
+  return finish_launch("route_experts", dtype == LC_F32    ? dispatch_route<float>(p, st)
+                                        : dtype == LC_BF16 ? dispatch_route<__nv_bfloat16>(p, st)
+                                                           : dispatch_route<__half>(p, st));
+}
+
+extern "C" int32_t lc_quantize_tokens(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ldx,
+                                      const int32_t* positions, int64_t copies, int64_t out_rows, const int32_t* valid,
+                                      int8_t* codes, int64_t ldq, float* scale, void* stream) {
+  if (rows < 0 || cols < 0 || ldx < cols || ldq < cols || (positions && copies < 1))
+    return fail(LC_ERR_INVALID_ARG, "quantize_tokens: bad shape");
+  if (!positions && out_rows < rows) return fail(LC_ERR_INVALID_ARG, "quantize_tokens: fewer output rows than rows");
+  if (dtype != LC_F32 && dtype != LC_BF16 && dtype != LC_F16)
+    return fail(LC_ERR_UNSUPPORTED, "quantize_tokens: dtype %d not supported", dtype);
+  if (rows == 0 || cols == 0) return LC_OK;
+  if (!x || !codes || !scale) return fail(LC_ERR_INVALID_ARG, "quantize_tokens: null pointer");
+  if (rows > 0x7fffffffLL || copies > 0x7fffffffLL) return fail(LC_ERR_UNSUPPORTED, "quantize_tokens: too many rows");
+  const TokenParams p = {x, rows, cols, ldx, positions, static_cast<int>(copies), out_rows, valid, codes, ldq, scale};
+  cudaStream_t st = as_stream(stream);
+  return finish_launch("quantize_tokens", dtype == LC_F32    ? launch_tokens<float>(p, st)
+                                          : dtype == LC_BF16 ? launch_tokens<__nv_bfloat16>(p, st)
+                                                             : launch_tokens<__half>(p, st));
+}
+
+extern "C" int32_t lc_combine_experts(const void* y, int32_t dtype, int64_t rows, int64_t cols, int64_t ldy,
+                                      const float* weights, const int32_t* positions, int64_t tokens, int64_t top_k,
+                                      const void* residual, int64_t ldr, void* out, int64_t ldo, void* stream) {
+  if (rows < 0 || cols < 0 || tokens < 0 || top_k < 1 || ldy < cols || ldo < cols || (residual && ldr < cols))
+    return fail(LC_ERR_INVALID_ARG, "combine_experts: bad shape");
+  if (dtype != LC_F32 && dtype != LC_BF16 && dtype != LC_F16)
+    return fail(LC_ERR_UNSUPPORTED, "combine_experts: dtype %d not supported", dtype);
+  if (tokens == 0 || cols == 0) return LC_OK;
+  if (!weights || !positions || !out || (!y && rows > 0)) return fail(LC_ERR_INVALID_ARG, "combine_experts: null pointer");
+  if (top_k > 0x7fffffffLL || cols > 0x7fffffffLL || tokens * cols > 0x7fffffffLL * 256)
+    return fail(LC_ERR_UNSUPPORTED, "combine_experts: too many elements");
+  const CombineParams p = {y, rows, cols, ldy, tokens, static_cast<int>(top_k), weights, positions, residual, ldr, out, ldo};
+  cudaStream_t st = as_stream(stream);
+  return finish_launch("combine_experts", dtype == LC_F32    ? launch_combine<float>(p, st)
+                                          : dtype == LC_BF16 ? launch_combine<__nv_bfloat16>(p, st)
+                                                             : launch_combine<__half>(p, st));
+}

@@ -22,6 +22,9 @@ static __typeof__(lc_dynamic_linear_f32)* p_dynamic_linear_f32;
 static __typeof__(lc_group_matmul_ex)* p_group_matmul_ex;
 static __typeof__(lc_wo_linear_s8_ex)* p_wo_linear_s8_ex;
 static __typeof__(lc_wo_swiglu_s8_ex)* p_wo_swiglu_s8_ex;
+static __typeof__(lc_expert_linear)* p_expert_linear;
+static __typeof__(lc_route_experts)* p_route_experts;
+static __typeof__(lc_combine_experts)* p_combine_experts;
 
 static inline int64_t as_int(PyObject* o) {
   if (o == Py_None) return 0;
@@ -93,6 +96,34 @@ static PyObject* f_wo_swiglu_s8_ex(PyObject* self, PyObject* const* args, Py_ssi
                                   (int32_t)A(12), P(13), A(14), P(15)));
 }
 
+static PyObject* f_expert_linear(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  int64_t iv[26];
+  double unused = 0.0;
+  if (n != 26 || !p_expert_linear) return unbound("expert_linear", 26, n, p_expert_linear != NULL);
+  if (!convert(args, n, -1, iv, &unused)) return NULL;
+  return finish(p_expert_linear(P(0), (int32_t)A(1), A(2), A(3), P(4), A(5), P(6), A(7), A(8), P(9), A(10), A(11), A(12),
+                                A(13), P(14), P(15), (int32_t)A(16), P(17), A(18), P(19), (int32_t)A(20), A(21), P(22),
+                                A(23), P(24), P(25)));
+}
+
+static PyObject* f_route_experts(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  int64_t iv[14];
+  double unused = 0.0;
+  if (n != 14 || !p_route_experts) return unbound("route_experts", 14, n, p_route_experts != NULL);
+  if (!convert(args, n, -1, iv, &unused)) return NULL;
+  return finish(p_route_experts(P(0), (int32_t)A(1), A(2), A(3), A(4), A(5), (int32_t)A(6), P(7), P(8), P(9), P(10), P(11),
+                                A(12), P(13)));
+}
+
+static PyObject* f_combine_experts(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  int64_t iv[14];
+  double unused = 0.0;
+  if (n != 14 || !p_combine_experts) return unbound("combine_experts", 14, n, p_combine_experts != NULL);
+  if (!convert(args, n, -1, iv, &unused)) return NULL;
+  return finish(p_combine_experts(P(0), (int32_t)A(1), A(2), A(3), A(4), P(5), P(6), A(7), A(8), P(9), A(10), P(11), A(12),
+                                  P(13)));
+}
+
 static PyObject* f_bind(PyObject* self, PyObject* args) {
   const char* name;
   unsigned long long address;
@@ -102,6 +133,9 @@ static PyObject* f_bind(PyObject* self, PyObject* args) {
   else if (!strcmp(name, "lc_group_matmul_ex")) p_group_matmul_ex = (__typeof__(p_group_matmul_ex))p;
   else if (!strcmp(name, "lc_wo_linear_s8_ex")) p_wo_linear_s8_ex = (__typeof__(p_wo_linear_s8_ex))p;
   else if (!strcmp(name, "lc_wo_swiglu_s8_ex")) p_wo_swiglu_s8_ex = (__typeof__(p_wo_swiglu_s8_ex))p;
+  else if (!strcmp(name, "lc_expert_linear")) p_expert_linear = (__typeof__(p_expert_linear))p;
+  else if (!strcmp(name, "lc_route_experts")) p_route_experts = (__typeof__(p_route_experts))p;
+  else if (!strcmp(name, "lc_combine_experts")) p_combine_experts = (__typeof__(p_combine_experts))p;
   else return PyErr_Format(PyExc_KeyError, "no fast binding for %s", name);
   Py_RETURN_NONE;
 }
@@ -112,6 +146,9 @@ static PyMethodDef methods[] = {
     {"group_matmul_ex", (PyCFunction)(void (*)(void))f_group_matmul_ex, METH_FASTCALL, "lc_group_matmul_ex"},
     {"wo_linear_s8_ex", (PyCFunction)(void (*)(void))f_wo_linear_s8_ex, METH_FASTCALL, "lc_wo_linear_s8_ex"},
     {"wo_swiglu_s8_ex", (PyCFunction)(void (*)(void))f_wo_swiglu_s8_ex, METH_FASTCALL, "lc_wo_swiglu_s8_ex"},
+    {"expert_linear", (PyCFunction)(void (*)(void))f_expert_linear, METH_FASTCALL, "lc_expert_linear"},
+    {"route_experts", (PyCFunction)(void (*)(void))f_route_experts, METH_FASTCALL, "lc_route_experts"},
+    {"combine_experts", (PyCFunction)(void (*)(void))f_combine_experts, METH_FASTCALL, "lc_combine_experts"},
     {NULL, NULL, 0, NULL}};
 
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fastcall", "low-overhead calls into liblucid_cuda", -1, methods};

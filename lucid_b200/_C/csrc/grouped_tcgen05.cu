@@ -1,0 +1,869 @@
+// int8 Linear of one or many groups with bias, activation and residual in its epilogue, for B200:
+//
+//   acc[m,n] = sum_k q[m,k] * w[e,n,k]                     e = group (expert) that owns row m
+//   out[m,n] = act(f32(acc - zx*wsum[e,n]) * sx[m] * sw[e,n] + bias[e,n]) + residual[m,n]
+//
+// The rows of q are sorted by group; offsets[e] .. offsets[e+1] are the rows of group e and live on the
+// device, so nothing of the routing is read on the host.  One group without offsets is the dense Linear.
+//
+// The WEIGHT is the 128-row (256-row in a CTA pair) operand of tcgen05.mma kind::i8 and the activation
+// codes are its N side, whose width follows the rows a tile really has (a multiple of 16, or 32 in a
+// pair): a group of three rows costs a 16-column product instead of a 128-row one, and one kernel serves
+// every group size.  The accumulator then has one output column per lane: scale, bias and zero-point
+// term of a lane are registers, the gate and up rows of a SwiGLU (interleaved in blocks of eight) sit
+// eight lanes apart in one warp, and a warp stores 32 adjacent outputs of a row at a time, so the
+// epilogue needs no transpose through shared memory.
+//
+// Two forms:
+//  * pair (cta_group::2): 256 weight rows x up to 256 rows of q per tile, each CTA of the pair loading
+//    its own 128 weight rows and half of the q rows; for groups that fill such tiles.
+//  * split (cta_group::1): 128 weight rows x up to 64 rows of q, K cut over the CTAs of a cluster.
+//    Decode batches have few tiles (a [4096, 14336] layer: 32), and a cluster of up to eight gives every
+//    SM a share of the weight's bytes.  The partial sums are int32, so adding them in rank 0's shared
+//    memory in any order gives the same bits.
+//
+// CTA = 320 threads: TMA warp, MMA warp, eight epilogue warps; the accumulator is double-buffered in
+// TMEM.  Every wait on an mbarrier is bounded: on expiry the role records a code in the status word and
+// leaves its loop, the CTA waits (bounded) for its own copies in flight, frees its TMEM and returns.
+#include <cuda.h>
+
+#include <mutex>
+
+#include "tcgen05.cuh"
+
+namespace lc {
+namespace grouped {
+
+using namespace tc;
+
+constexpr int BK = 128;               // bytes of K per stage = one 128B swizzle atom
+constexpr int UMMA_K = 32;
+constexpr int WROWS = 128;            // weight rows a CTA loads per tile
+constexpr int A_BYTES = WROWS * BK;
+constexpr int NUM_THREADS = 320;
+constexpr int EPI_WARPS = 8;
+constexpr int EPI_THREADS = EPI_WARPS * 32;
+constexpr int MAX_GROUPS = 1024;
+
+template <int CG>
+struct Cfg;
+template <>
+struct Cfg<2> {
+  static constexpr int kTile = 256;   // weight rows per tile
+  static constexpr int kTokens = 256; // q rows per tile
+  static constexpr int kStep = 32;    // granularity of the instruction's N
+  static constexpr int kBox = 32;     // q rows per TMA box
+  static constexpr int kStages = 6;
+  static constexpr int kBBytes = (kTokens / 2) * BK;
+  static constexpr int kChunk = 32;   // accumulator columns an epilogue warp takes at a time
+  static constexpr int kRedBytes = 0;
+};
+template <>
+struct Cfg<1> {
+  static constexpr int kTile = 128;
+  static constexpr int kTokens = 64;
+  static constexpr int kStep = 16;
+  static constexpr int kBox = 16;
+  static constexpr int kStages = 7;
+  static constexpr int kBBytes = kTokens * BK;
+  static constexpr int kChunk = 16;
+  static constexpr int kRedBytes = kTokens * WROWS * 4;  // partial sums of the other ranks, [column][lane]
+};
+template <int CG>
+__host__ __device__ constexpr int stage_bytes() { return A_BYTES + Cfg<CG>::kBBytes; }
+template <int CG>
+__host__ __device__ constexpr int smem_bytes() {
+  return 1024 + Cfg<CG>::kStages * stage_bytes<CG>() + 256 + Cfg<CG>::kRedBytes + 2 * Cfg<CG>::kTokens * 4 +
+         2 * (MAX_GROUPS + 1) * 4;
+}
+static_assert(smem_bytes<1>() <= 232448 && smem_bytes<2>() <= 232448, "shared memory of a CTA");
+
+enum : int { ST_PRODUCER = 1, ST_MMA = 2, ST_EPILOGUE = 3 };
+
+struct Params {
+  int64_t R, N, K;          // rows of q, weight rows of a group, contraction length
+  int E;
+  const int32_t* offsets;   // [E + 1] or null (one group of R rows)
+  const float* sx;          // 1 or R
+  int sx_per_row;
+  const float* zx;          // device scalar holding an integer value, or null
+  const int32_t* wsum;      // [E, N], with zx
+  const float* sw;          // [E, N]
+  const float* bias;        // [E, N] or null
+  int act;
+  const void* residual;     // [R, out columns] of out's type, or null
+  int64_t ldr;
+  void* out;
+  int out_dtype;
+  int64_t ldo;
+  int32_t* status;
+  int wait_test;
+  int split;                // CTAs of a cluster that share a tile's K (CG == 1)
+  int early_weights;        // the weight and offsets were complete before the previous kernel began
+  uint32_t idesc;           // instruction descriptor without its N field
+};
+
+__device__ __forceinline__ void report(int32_t* status, int code) {
+  if (status) atomicCAS(status, 0, code);
+}
+
+// ---- cluster-scope synchronisation of the split form -------------------------------------
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, long long budget) {
+  if (mbar_try_wait_cluster(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_wait_cluster(bar, parity)) {
+    if (clock64() - t0 > budget) return false;
+  }
+  return true;
+}
+__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ void red_add_cluster(uint32_t cluster_addr, uint32_t v) {
+  asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                                 uint32_t cluster_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(cluster_bar)
+      : "memory");
+}
+__device__ __forceinline__ void tc_ld(uint32_t taddr, uint32_t (&r)[32]) { tc_ld_32x32(taddr, r); }
+__device__ __forceinline__ void tc_ld(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+// barrier over the epilogue threads that also ANDs a predicate
+__device__ __forceinline__ bool epilogue_all(bool ok) {
+  uint32_t out;
+  asm volatile(
+      "{\n\t.reg .pred pin, pout;\n\t"
+      "setp.ne.u32 pin, %1, 0;\n\t"
+      "bar.red.and.pred pout, 1, %2, pin;\n\t"
+      "selp.u32 %0, 1, 0, pout;\n\t}"
+      : "=r"(out)
+      : "r"(static_cast<uint32_t>(ok)), "n"(EPI_THREADS)
+      : "memory");
+  return out != 0;
+}
+
+// ---- which tile ---------------------------------------------------------------------------
+struct Tile {
+  int e, m0, rows;  // group, first row of q, rows
+  int64_t n0;       // first weight row inside the group
+};
+
+// Tiles are numbered group by group; within a group, bands of 16 row tiles share the weight tiles.  The walk
+// only moves forward because a CTA's tile numbers grow.
+template <int CG>
+struct TileWalk {
+  const int* start;  // [E + 1] first tile of each group
+  const int* off;    // [E + 1] first row of each group
+  int tiles_n, e;
+  __device__ __forceinline__ TileWalk(const int* s, const int* o, int tn) : start(s), off(o), tiles_n(tn), e(0) {}
+  __device__ __forceinline__ Tile at(int t) {
+    while (t >= start[e + 1]) ++e;
+    const int rows = off[e + 1] - off[e];
+    const int tiles_m = (rows + Cfg<CG>::kTokens - 1) / Cfg<CG>::kTokens;
+    const int local = t - start[e];
+    constexpr int kBand = 16;
+    const int band = kBand * tiles_n;
+    const int g = local / band, first = g * kBand;
+    const int gm = tiles_m - first < kBand ? tiles_m - first : kBand;
+    const int r = local - g * band;
+    const int tm = first + r % gm, tn = r / gm;
+    Tile tile;
+    tile.e = e;
+    tile.m0 = off[e] + tm * Cfg<CG>::kTokens;
+    const int left = off[e + 1] - tile.m0;
+    tile.rows = left < Cfg<CG>::kTokens ? left : Cfg<CG>::kTokens;
+    tile.n0 = static_cast<int64_t>(tn) * Cfg<CG>::kTile;
+    return tile;
+  }
+};
+
+// ---- epilogue arithmetic -------------------------------------------------------------------
+// EXACT for fp32 results (library expf and IEEE division); 16-bit results take the hardware exponential and
+// the approximate division, whose relative errors (below 2^-20 for the arguments that matter) vanish in the
+// rounding to 8 or 11 bits.
+template <bool EXACT>
+__device__ __forceinline__ float sigmoid_times(float v, float arg) {  // v / (1 + exp(-arg))
+  if (EXACT) return __fdiv_rn(v, 1.0f + expf(-arg));
+  return __fdividef(v, 1.0f + __expf(-arg));
+}
+template <bool EXACT>
+__device__ __forceinline__ float activate(float v, int act) {
+  switch (act) {
+    case LC_ACT_RELU: return v < 0.0f ? 0.0f : v;  // NaN compares false and stays
+    case LC_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678118654752440f));
+    case LC_ACT_GELU_TANH:  // 0.5 v (1 + tanh(u)) = v / (1 + exp(-2u)), u = sqrt(2/pi) (v + 0.044715 v^3)
+      return sigmoid_times<EXACT>(v, 1.5957691216057307f * (v + 0.044715f * v * v * v));
+    case LC_ACT_SILU: return sigmoid_times<EXACT>(v, v);
+    default: return v;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float widen(T v);
+template <>
+__device__ __forceinline__ float widen<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float widen<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float widen<__half>(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T narrow(float v);
+template <>
+__device__ __forceinline__ float narrow<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
+
+// One chunk of CH accumulator columns: this lane's output column `n` of the rows row0 .. row0 + rows - 1.
+template <typename T, int CH>
+__device__ __forceinline__ void finish_chunk(const Params& p, const uint32_t (&r)[CH], int64_t row0, int rows,
+                                             int64_t n, int lane, const float* sx, float sw, float bias, int corr) {
+  constexpr bool kExact = sizeof(T) == 4;
+  float f[CH];
+#pragma unroll
+  for (int j = 0; j < CH; j += 4) {
+    const float4 s = *reinterpret_cast<const float4*>(sx + j);
+    const float sv[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      f[j + i] = __fadd_rn(__fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(r[j + i]) - corr), sv[i]), sw), bias);
+  }
+  if (p.act == LC_ACT_SWIGLU) {
+    // lanes 8 apart hold the gate and up value of one unit: each finishes every other row
+    const int up = (lane >> 3) & 1;
+    const int64_t unit = ((n >> 4) << 3) | (n & 7);
+    T* o = static_cast<T*>(p.out) + (row0 + up) * p.ldo + unit;
+    const T* res = static_cast<const T*>(p.residual) + (p.residual ? (row0 + up) * p.ldr + unit : 0);
+#pragma unroll
+    for (int j = 0; j < CH; j += 2) {
+      const float got = __shfl_xor_sync(0xffffffffu, up ? f[j] : f[j + 1], 8);
+      const float gate = up ? got : f[j], lin = up ? f[j + 1] : got;
+      float v = sigmoid_times<kExact>(gate, gate) * lin;
+      if (j + up < rows && n < p.N) {
+        if (p.residual) v += widen<T>(res[j * p.ldr]);
+        o[j * p.ldo] = narrow<T>(v);
+      }
+    }
+    return;
+  }
+  if (p.act != LC_ACT_NONE) {
+#pragma unroll
+    for (int j = 0; j < CH; ++j) f[j] = activate<kExact>(f[j], p.act);
+  }
+  if (n >= p.N) return;
+  if (p.residual) {
+    const T* res = static_cast<const T*>(p.residual) + row0 * p.ldr + n;
+    T v[CH];
+#pragma unroll
+    for (int j = 0; j < CH; ++j)
+      if (j < rows) v[j] = res[j * p.ldr];
+#pragma unroll
+    for (int j = 0; j < CH; ++j)
+      if (j < rows) f[j] += widen<T>(v[j]);
+  }
+  T* o = static_cast<T*>(p.out) + row0 * p.ldo + n;
+#pragma unroll
+  for (int j = 0; j < CH; ++j)
+    if (j < rows) o[j * p.ldo] = narrow<T>(f[j]);
+}
+
+template <int CH>
+__device__ __forceinline__ void finish(const Params& p, const uint32_t (&r)[CH], int64_t row0, int rows, int64_t n,
+                                       int lane, const float* sx, float sw, float bias, int corr) {
+  if (p.out_dtype == LC_F32)
+    finish_chunk<float, CH>(p, r, row0, rows, n, lane, sx, sw, bias, corr);
+  else if (p.out_dtype == LC_BF16)
+    finish_chunk<__nv_bfloat16, CH>(p, r, row0, rows, n, lane, sx, sw, bias, corr);
+  else
+    finish_chunk<__half, CH>(p, r, row0, rows, n, lane, sx, sw, bias, corr);
+}
+
+template <int CG>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_q,
+                      const Params p) {
+  using C = Cfg<CG>;
+  constexpr int STAGES = C::kStages, STAGE_BYTES = stage_bytes<CG>(), CH = C::kChunk;
+  constexpr int TMEM_COLS = 2 * C::kTokens;  // 512 or 128
+  static_assert(2 * STAGES * 8 + 6 * 8 <= 256, "barrier area");
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint32_t s_tmem_base;
+
+  pdl_launch_dependents();
+  const uint32_t tiles_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t bar_base = tiles_base + STAGES * STAGE_BYTES;
+  const uint32_t red_base = bar_base + 256;
+  uint8_t* const after = smem_raw + (red_base - smem_u32(smem_raw));
+  int* const s_red = reinterpret_cast<int*>(after);
+  float* const s_sx = reinterpret_cast<float*>(after + C::kRedBytes);  // two accumulator stages
+  int* const s_off = reinterpret_cast<int*>(s_sx + 2 * C::kTokens);
+  int* const s_start = s_off + (MAX_GROUPS + 1);
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
+  auto acc_full_bar = [&](int s) { return bar_base + 8u * (2 * STAGES + s); };
+  auto acc_empty_bar = [&](int s) { return bar_base + 8u * (2 * STAGES + 2 + s); };
+  const uint32_t part_bar = bar_base + 8u * (2 * STAGES + 4);  // rank 0: the other ranks' sums have been added
+  const uint32_t free_bar = part_bar + 8u;                     // other ranks: rank 0's buffer is zero again
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long budget = p.wait_test ? 20000LL : kWaitCycles;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int cluster = CG == 2 ? 2 : p.split;
+  const int unit = static_cast<int>(blockIdx.x) / cluster, units = static_cast<int>(gridDim.x) / cluster;
+  const int tiles_n = static_cast<int>((p.N + C::kTile - 1) / C::kTile);
+  const int num_kb = static_cast<int>((p.K + BK - 1) / BK);
+  const int kb0 = CG == 2 ? 0 : static_cast<int>(static_cast<int64_t>(num_kb) * rank / p.split);
+  const int kb1 = CG == 2 ? num_kb : static_cast<int>(static_cast<int64_t>(num_kb) * (rank + 1) / p.split);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(acc_full_bar(s), 1);
+      mbar_init(acc_empty_bar(s), CG * EPI_WARPS);
+    }
+    mbar_init(part_bar, p.split > 1 ? (p.split - 1) * EPI_WARPS : 1);
+    mbar_init(free_bar, EPI_WARPS);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    if constexpr (CG == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)),
+                   "r"(static_cast<uint32_t>(TMEM_COLS))
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)),
+                   "r"(static_cast<uint32_t>(TMEM_COLS))
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+  }
+  if (C::kRedBytes > 0 && p.split > 1 && leader)
+    for (int i = threadIdx.x; i < C::kRedBytes / 4; i += NUM_THREADS) s_red[i] = 0;
+
+  if (!p.early_weights) pdl_wait();
+  // first row and first tile of every group (clamped to the rows there are: offsets come from the caller)
+  if (warp == 2) {
+    if (!p.offsets) {
+      if (lane == 0) {
+        s_off[0] = 0;
+        s_off[1] = static_cast<int>(p.R);
+        s_start[0] = 0;
+        s_start[1] = static_cast<int>((p.R + C::kTokens - 1) / C::kTokens) * tiles_n;
+      }
+    } else {
+      const int R = static_cast<int>(p.R);
+      int base = 0;
+      for (int e0 = 0; e0 < p.E; e0 += 32) {
+        const int e = e0 + lane;
+        int tiles = 0;
+        if (e < p.E) {
+          const int a = min(max(p.offsets[e], 0), R), b = min(max(p.offsets[e + 1], a), R);
+          tiles = (b - a + C::kTokens - 1) / C::kTokens * tiles_n;
+          s_off[e] = a;
+          if (e == p.E - 1) s_off[p.E] = b;
+        }
+        int sum = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += v;
+        }
+        if (e < p.E) s_start[e + 1] = base + sum;
+        base += __shfl_sync(0xffffffffu, sum, 31);
+      }
+      if (lane == 0) s_start[0] = 0;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // the other CTAs' barriers (and rank 0's zeroed buffer) exist before anything reaches them
+  tc_fence_after();
+  const uint32_t tmem_base = s_tmem_base;
+  const int total = s_start[p.E];
+
+  if (warp == 0) {
+    // ===================== TMA producer =====================
+    if (lane == 0) {
+      uint32_t armed_parity[STAGES];
+      bool armed[STAGES];
+      for (int s = 0; s < STAGES; ++s) armed[s] = false;
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true, waited = !p.early_weights;
+      TileWalk<CG> walk(s_start, s_off, tiles_n);
+      for (int t = unit; t < total && ok && !p.wait_test; t += units) {
+        const Tile tile = walk.at(t);
+        const int cols = (tile.rows + C::kStep - 1) / C::kStep * C::kStep;
+        const int mine = cols / CG;  // q rows this CTA loads
+        const int boxes = (mine + C::kBox - 1) / C::kBox;
+        const uint32_t bytes = CG * (A_BYTES + boxes * C::kBox * BK);
+        const int n0 = static_cast<int>(tile.n0) + (CG == 2 ? static_cast<int>(rank) * WROWS : 0);
+        const int m0 = tile.m0 + (CG == 2 ? static_cast<int>(rank) * mine : 0);
+        auto arm = [&](int s) {
+          if (CG == 1 || leader) {
+            mbar_expect_tx(full_bar(s), bytes);
+            armed[s] = true;
+          }
+        };
+        auto load_w = [&](int s, int kb) {
+          const uint32_t dst = tiles_base + s * STAGE_BYTES;
+          if constexpr (CG == 2)
+            tma_load_3d_pair(dst, &tmap_w, kb * BK, n0, tile.e, map_to_cta(full_bar(s), 0));
+          else
+            tma_load_3d(dst, &tmap_w, kb * BK, n0, tile.e, full_bar(s));
+        };
+        auto load_q = [&](int s, int kb) {
+          const uint32_t dst = tiles_base + s * STAGE_BYTES + A_BYTES;
+          for (int b = 0; b < boxes; ++b) {
+            if constexpr (CG == 2)
+              tma_load_2d_pair(dst + b * C::kBox * BK, &tmap_q, kb * BK, m0 + b * C::kBox, map_to_cta(full_bar(s), 0));
+            else
+              tma_load_2d(dst + b * C::kBox * BK, &tmap_q, kb * BK, m0 + b * C::kBox, full_bar(s));
+          }
+        };
+        int kb = kb0;
+        if (!waited) {
+          // the ring is empty: fill it with weights while the kernel before this one still writes the codes
+          const int ahead = min(STAGES, kb1 - kb0);
+          for (int s = 0; s < ahead; ++s) {
+            arm(s);
+            armed_parity[s] = 0;
+            load_w(s, kb0 + s);
+          }
+          pdl_wait();
+          waited = true;
+          for (int s = 0; s < ahead; ++s) load_q(s, kb0 + s);
+          kb = kb0 + ahead;
+          stage = ahead % STAGES;
+          phase = ahead == STAGES ? 1u : 0u;
+        }
+        for (; kb < kb1; ++kb) {
+          if (!mbar_wait(empty_bar(stage), phase ^ 1u, budget)) {
+            report(p.status, ST_PRODUCER);
+            ok = false;
+            break;
+          }
+          arm(stage);
+          armed_parity[stage] = phase;
+          load_w(stage, kb);
+          load_q(stage, kb);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      // do not leave while a bulk copy may still be landing (a pair's leader counts the bytes of both CTAs)
+      for (int s = 0; s < STAGES; ++s)
+        if (armed[s]) mbar_wait(full_bar(s), armed_parity[s]);
+    }
+  } else if (warp == 1) {
+    // ===================== MMA issuer (a pair's leader only) =====================
+    if ((CG == 1 || leader) && lane == 0) {
+      int stage = 0, it = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      TileWalk<CG> walk(s_start, s_off, tiles_n);
+      for (int t = unit; t < total && ok; t += units, ++it) {
+        const Tile tile = walk.at(t);
+        const uint32_t cols = (tile.rows + C::kStep - 1) / C::kStep * C::kStep;
+        const uint32_t idesc = p.idesc | ((cols >> 3) << 17);
+        const int as = it & 1;
+        if (!mbar_wait(acc_empty_bar(as), ((it >> 1) & 1) ^ 1u, budget)) {
+          report(p.status, ST_MMA);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(as * C::kTokens);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(full_bar(stage), phase, budget)) {
+            report(p.status, ST_MMA);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t src = tiles_base + stage * STAGE_BYTES;
+          const uint64_t w_desc = make_smem_desc(src), q_desc = make_smem_desc(src + A_BYTES);
+#pragma unroll
+          for (int j = 0; j < BK / UMMA_K; ++j) {
+            const uint64_t koff = static_cast<uint64_t>((j * UMMA_K) >> 4);
+            const uint32_t accumulate = (kb != kb0 || j != 0) ? 1u : 0u;
+            if constexpr (CG == 2)
+              tc_mma_i8_pair(d_tmem, w_desc + koff, q_desc + koff, idesc, accumulate);
+            else
+              tc_mma_i8(d_tmem, w_desc + koff, q_desc + koff, idesc, accumulate);
+          }
+          if constexpr (CG == 2)
+            tc_commit_pair(empty_bar(stage));
+          else
+            tc_commit(empty_bar(stage));
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (ok) {
+          if constexpr (CG == 2)
+            tc_commit_pair(acc_full_bar(as));
+          else
+            tc_commit(acc_full_bar(as));
+        }
+      }
+    }
+  } else {
+    // ===================== epilogue (eight warps of every CTA) =====================
+    const int q = warp & 3;  // TMEM lane quadrant this warp may read
+    const int group = (warp - 2) >> 2;
+    const int et = threadIdx.x - 64;
+    if (p.early_weights) pdl_wait();
+    const int zx = p.zx ? __float2int_rn(__ldg(p.zx)) : 0;
+    TileWalk<CG> walk(s_start, s_off, tiles_n);
+    int it = 0;
+    for (int t = unit; t < total; t += units, ++it) {
+      const Tile tile = walk.at(t);
+      const int as = it & 1;
+      float* const sx = s_sx + as * C::kTokens;
+      if (et < C::kTokens) sx[et] = et < tile.rows ? __ldg(p.sx + (p.sx_per_row ? tile.m0 + et : 0)) : 0.0f;
+      const int64_t n = tile.n0 + (CG == 2 ? static_cast<int64_t>(rank) * WROWS : 0) + q * 32 + lane;
+      const int64_t at = static_cast<int64_t>(tile.e) * p.N + n;
+      const bool in = n < p.N;
+      const float sw = in ? __ldg(p.sw + at) : 0.0f;
+      const float bias = (in && p.bias) ? __ldg(p.bias + at) : 0.0f;
+      const int corr = (in && p.wsum) ? zx * __ldg(p.wsum + at) : 0;
+      bool arrived = mbar_wait(acc_full_bar(as), (it >> 1) & 1, budget);
+      if (CG == 1 && p.split > 1)
+        arrived = arrived && (leader ? mbar_wait_cluster(part_bar, it & 1, budget)
+                                     : mbar_wait_cluster(free_bar, (it & 1) ^ 1u, budget));
+      // also publishes the staged scales; those of the tile before last are no longer read
+      if (!epilogue_all(arrived)) {
+        report(p.status, ST_EPILOGUE);
+        break;
+      }
+      tc_fence_after();
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(as * C::kTokens);
+#pragma unroll 1
+      for (int c = group * CH; c < tile.rows; c += 2 * CH) {
+        uint32_t r[CH];
+        tc_ld(t_row + static_cast<uint32_t>(c), r);
+        tc_wait_ld();
+        if (CG == 1 && p.split > 1) {
+          const uint32_t slot = static_cast<uint32_t>((c * WROWS + q * 32 + lane) * 4);
+          if (!leader) {
+            const uint32_t dst = map_to_cta(red_base, 0) + slot;
+#pragma unroll
+            for (int j = 0; j < CH; ++j)
+              if (c + j < tile.rows) red_add_cluster(dst + j * WROWS * 4, r[j]);
+            continue;
+          }
+          int* const mine = s_red + slot / 4;
+#pragma unroll
+          for (int j = 0; j < CH; ++j) {
+            if (c + j < tile.rows) {
+              r[j] += static_cast<uint32_t>(mine[j * WROWS]);
+              mine[j * WROWS] = 0;
+            }
+          }
+        }
+        const int left = tile.rows - c;
+        finish<CH>(p, r, tile.m0 + c, left < CH ? left : CH, n, lane, sx + c, sw, bias, corr);
+      }
+      tc_fence_before();
+      if (CG == 1 && p.split > 1) {
+        asm volatile("fence.acq_rel.cluster;" ::: "memory");
+        __syncwarp();
+        if (!leader) {
+          if (lane == 0) mbar_arrive_release_cluster(map_to_cta(part_bar, 0));
+        } else if (lane > 0 && lane < p.split) {
+          mbar_arrive_release_cluster(map_to_cta(free_bar, lane));
+        }
+      }
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CG == 2)
+          mbar_arrive_cluster(map_to_cta(acc_empty_bar(as), 0));
+        else
+          mbar_arrive(acc_empty_bar(as));
+      }
+    }
+    // rows behind the last group belong to no group: zero
+    if (p.offsets) {
+      const int64_t width = p.act == LC_ACT_SWIGLU ? p.N / 2 : p.N;
+      for (int64_t row = s_off[p.E] + static_cast<int64_t>(blockIdx.x); row < p.R; row += gridDim.x)
+        for (int64_t c = et; c < width; c += EPI_THREADS) {
+          if (p.out_dtype == LC_F32)
+            static_cast<float*>(p.out)[row * p.ldo + c] = 0.0f;
+          else
+            static_cast<uint16_t*>(p.out)[row * p.ldo + c] = 0;
+        }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // no CTA frees TMEM or leaves while another may still reach its memory
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    if constexpr (CG == 2)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),
+                   "r"(static_cast<uint32_t>(TMEM_COLS))
+                   : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),
+                   "r"(static_cast<uint32_t>(TMEM_COLS))
+                   : "memory");
+  }
+}
+
+// ---- host side -------------------------------------------------------------------------------
+struct DeviceInfo {
+  cudaError_t err;
+  int clusters[4];  // resident clusters of 1, 2, 4, 8 CTAs of the split form
+};
+
+static cudaError_t launch_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attrs, unsigned grid, int smem,
+                                 int cluster, cudaStream_t st) {
+  *cfg = {};
+  cfg->gridDim = dim3(grid);
+  cfg->blockDim = dim3(NUM_THREADS);
+  cfg->dynamicSmemBytes = smem;
+  cfg->stream = st;
+  attrs[0].id = cudaLaunchAttributeClusterDimension;
+  attrs[0].val.clusterDim.x = cluster;
+  attrs[0].val.clusterDim.y = 1;
+  attrs[0].val.clusterDim.z = 1;
+  attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg->attrs = attrs;
+  cfg->numAttrs = 2;
+  return cudaSuccess;
+}
+
+static int32_t device_info(const DeviceInfo** out) {
+  constexpr int kMaxDevices = 64;
+  static std::once_flag flags[kMaxDevices];
+  static DeviceInfo infos[kMaxDevices];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices)
+    return fail(LC_ERR_CUDA, "no current CUDA device");
+  std::call_once(flags[dev], [dev]() {
+    DeviceInfo& info = infos[dev];
+    info.err = cudaFuncSetAttribute(grouped_linear_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<1>());
+    if (info.err == cudaSuccess)
+      info.err = cudaFuncSetAttribute(grouped_linear_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<2>());
+    const int sms = sm_count();
+    for (int i = 0; i < 4 && info.err == cudaSuccess; ++i) {
+      cudaLaunchConfig_t cfg;
+      cudaLaunchAttribute attrs[2];
+      launch_config(&cfg, attrs, static_cast<unsigned>(sms / (1 << i) << i), smem_bytes<1>(), 1 << i, nullptr);
+      cfg.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, grouped_linear_kernel<1>, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        n = i == 0 ? sms : 0;
+      }
+      info.clusters[i] = n;
+    }
+  });
+  if (infos[dev].err != cudaSuccess)
+    return fail(LC_ERR_CUDA, "grouped_linear: cannot reserve shared memory: %s", cudaGetErrorString(infos[dev].err));
+  *out = &infos[dev];
+  return LC_OK;
+}
+
+// Groups whose mean row count exceeds this take the pair form.
+constexpr int64_t kPairRows = 64;
+
+static int32_t launch(const void* q, int64_t ldq, const int8_t* w, int64_t ldw, int64_t group_stride, int q_unsigned,
+                      Params& p, int variant, cudaStream_t st) {
+  const DeviceInfo* info = nullptr;
+  if (int32_t rc = device_info(&info)) return rc;
+  const int64_t sms = sm_count();
+  const bool pair = variant == 2 || (variant == 0 && p.R > kPairRows * p.E);
+  CUtensorMap map_w, map_q;
+  if (int32_t rc = encode_tensor_map_3d(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, p.K, p.N, p.E, ldw, group_stride, BK,
+                                        WROWS, CU_TENSOR_MAP_SWIZZLE_128B))
+    return rc;
+  if (int32_t rc = encode_tensor_map_2d(&map_q, CU_TENSOR_MAP_DATA_TYPE_UINT8, q, p.K, p.R, ldq, BK,
+                                        pair ? Cfg<2>::kBox : Cfg<1>::kBox, CU_TENSOR_MAP_SWIZZLE_128B))
+    return rc;
+  // kind::i8: D s32 (2) in bits [4,6); A (weight, s8 = 1) in [7,10), B (codes, s8 = 1 or u8 = 0) in [10,13); both
+  // K-major; N >> 3 in [17,23) is filled in per tile; M >> 4 in [24,29)
+  p.idesc = (2u << 4) | (1u << 7) | ((q_unsigned ? 0u : 1u) << 10) |
+            (static_cast<uint32_t>((pair ? 256 : 128) >> 4) << 24);
+  const int64_t tile_n = pair ? 256 : 128, tile_m = pair ? 256 : 64;
+  const int64_t tiles_n = (p.N + tile_n - 1) / tile_n;
+  // upper bound of the tiles there can be: one partly filled row tile per group that has rows
+  const int64_t groups = p.offsets ? (p.E < p.R ? p.E : p.R) : 1;
+  const int64_t tiles = tiles_n * ((p.R - groups) / tile_m + groups);
+  if (tiles > 0x7fffffffLL) return fail(LC_ERR_UNSUPPORTED, "grouped_linear: too many tiles");
+  int cluster = 2;
+  int64_t units = sms / 2;
+  p.split = 1;
+  if (!pair) {
+    // K split: the waves of tiles over the clusters that fit, times each CTA's share of K; two K blocks of
+    // hand-over are charged per split tile
+    const int num_kb = static_cast<int>((p.K + BK - 1) / BK);
+    double best = 0.0;
+    cluster = 1;
+    for (int i = 0; i < 4; ++i) {
+      const int s = 1 << i;
+      if (info->clusters[i] < 1 || num_kb < 4 * s) break;
+      const int64_t waves = (tiles + info->clusters[i] - 1) / info->clusters[i];
+      const double cost = static_cast<double>(waves) * ((num_kb + s - 1) / s + (s > 1 ? 2 : 0));
+      if (i == 0 || cost < best) {
+        best = cost;
+        cluster = s;
+        units = info->clusters[i];
+      }
+    }
+    p.split = cluster;
+  }
+  if (units > tiles) units = tiles;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attrs[2];
+  launch_config(&cfg, attrs, static_cast<unsigned>(units * cluster), pair ? smem_bytes<2>() : smem_bytes<1>(), cluster, st);
+  const cudaError_t err = pair ? cudaLaunchKernelEx(&cfg, grouped_linear_kernel<2>, map_w, map_q, p)
+                               : cudaLaunchKernelEx(&cfg, grouped_linear_kernel<1>, map_w, map_q, p);
+  if (err != cudaSuccess) return fail(LC_ERR_CUDA, "grouped_linear: %s", cudaGetErrorString(err));
+  return check_launch("grouped_linear");
+}
+
+static int32_t check_and_launch(const char* what, const void* q, int q_unsigned, int64_t ldq, int64_t R,
+                                const int32_t* offsets, int64_t E, const int8_t* w, int64_t ldw, int64_t group_stride,
+                                int64_t N, int64_t K, const float* sx, int sx_per_row, const float* zx,
+                                const int32_t* wsum, const float* sw, const float* bias, int act, const void* residual,
+                                int64_t ldr, void* out, int out_dtype, int64_t ldo, int32_t* status, int variant,
+                                int early_weights, cudaStream_t st) {
+  const int wait_test = (variant & LC_QLINEAR_WAIT_TEST) ? 1 : 0;
+  variant &= ~LC_QLINEAR_WAIT_TEST;
+  if (wait_test && !status) return fail(LC_ERR_INVALID_ARG, "%s: the wait test needs a status word", what);
+  if (variant < 0 || variant > 2) return fail(LC_ERR_INVALID_ARG, "%s: variant must be 0, 1 or 2", what);
+  if (R < 0 || N < 0 || K <= 0 || E < 1) return fail(LC_ERR_INVALID_ARG, "%s: bad shape", what);
+  if (act < LC_ACT_NONE || act > LC_ACT_SWIGLU) return fail(LC_ERR_INVALID_ARG, "%s: unknown activation %d", what, act);
+  if (act == LC_ACT_SWIGLU && N % 16)
+    return fail(LC_ERR_INVALID_ARG, "%s: swiglu needs weight rows in interleaved blocks of 8 gate and 8 up rows", what);
+  if (out_dtype != LC_F32 && out_dtype != LC_BF16 && out_dtype != LC_F16)
+    return fail(LC_ERR_UNSUPPORTED, "%s: out_dtype %d not supported", what, out_dtype);
+  if (!offsets && E != 1) return fail(LC_ERR_INVALID_ARG, "%s: more than one group needs offsets", what);
+  if (E > MAX_GROUPS) return fail(LC_ERR_UNSUPPORTED, "%s: at most %d groups", what, MAX_GROUPS);
+  if (R == 0 || N == 0) return LC_OK;
+  if (!q || !w || !sx || !sw || !out) return fail(LC_ERR_INVALID_ARG, "%s: null pointer", what);
+  if ((zx == nullptr) != (wsum == nullptr)) return fail(LC_ERR_INVALID_ARG, "%s: zx and wsum go together", what);
+  const int64_t width = act == LC_ACT_SWIGLU ? N / 2 : N;
+  if (ldq < K || ldw < K || ldo < width || (residual && ldr < width) || (E > 1 && group_stride < N * ldw - (ldw - K)))
+    return fail(LC_ERR_INVALID_ARG, "%s: leading dimension too small", what);
+  if (ldq % 16 || ldw % 16 || (E > 1 && group_stride % 16) || !aligned(q, 16) || !aligned(w, 16))
+    return fail(LC_ERR_UNSUPPORTED, "%s: operand rows must start on 16-byte boundaries (pad ldq / ldw to 16)", what);
+  // |sum| <= K * 255 * 128 must stay inside int32; rows and columns inside the TMA coordinate range
+  if (K > 65536) return fail(LC_ERR_UNSUPPORTED, "%s: K above 65536 could overflow int32", what);
+  if (R > 0x7fffffffLL - 512 || N > 0x7fffffffLL - 512) return fail(LC_ERR_UNSUPPORTED, "%s: dimension too large", what);
+  Params p = {};
+  p.R = R;
+  p.N = N;
+  p.K = K;
+  p.E = static_cast<int>(E);
+  p.offsets = offsets;
+  p.sx = sx;
+  p.sx_per_row = sx_per_row;
+  p.zx = zx;
+  p.wsum = wsum;
+  p.sw = sw;
+  p.bias = bias;
+  p.act = act;
+  p.residual = residual;
+  p.ldr = ldr;
+  p.out = out;
+  p.out_dtype = out_dtype;
+  p.ldo = ldo;
+  p.status = status;
+  p.wait_test = wait_test;
+  p.early_weights = early_weights;
+  return launch(q, ldq, w, ldw, E > 1 ? group_stride : N * ldw, q_unsigned, p, variant, st);
+}
+
+}  // namespace grouped
+}  // namespace lc
+
+using namespace lc;
+
+extern "C" int32_t lc_grouped_qlinear_i8(const void* q, int32_t q_unsigned, int64_t ldq, int64_t rows,
+                                         const int32_t* offsets, int64_t groups, const int8_t* wq, int64_t ldw,
+                                         int64_t group_stride, int64_t N, int64_t K, const float* sx,
+                                         int32_t sx_per_row, const float* zx, const int32_t* wsum, const float* sw,
+                                         const float* bias, int32_t activation, const void* residual, int64_t ldr,
+                                         void* out, int32_t out_dtype, int64_t ldo, int32_t* status, int32_t variant,
+                                         void* stream) {
+  return grouped::check_and_launch("grouped_qlinear_i8", q, q_unsigned, ldq, rows, offsets, groups, wq, ldw,
+                                   group_stride, N, K, sx, sx_per_row, zx, wsum, sw, bias, activation, residual, ldr,
+                                   out, out_dtype, ldo, status, variant, 0, as_stream(stream));
+}
+
+// ---- quantization of the activations and the product as one call --------------------------------
+static inline int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
+static inline int64_t pad16(int64_t k) { return (k + 15) / 16 * 16; }
+
+extern "C" int64_t lc_expert_linear_workspace_bytes(int64_t rows, int64_t K) {
+  if (rows < 0 || K <= 0) return 0;
+  return round256(rows * pad16(K)) + round256(rows * 4);  // codes, one scale per row
+}
+
+extern "C" int32_t lc_expert_linear(const void* x, int32_t x_dtype, int64_t x_rows, int64_t ldx,
+                                    const int32_t* positions, int64_t top_k, const int32_t* offsets, int64_t groups,
+                                    int64_t rows, const int8_t* wq, int64_t ldw, int64_t group_stride, int64_t N,
+                                    int64_t K, const float* sw, const float* bias, int32_t activation,
+                                    const void* residual, int64_t ldr, void* out, int32_t out_dtype, int64_t ldo,
+                                    void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
+  if (rows < 0 || K <= 0 || N < 0) return fail(LC_ERR_INVALID_ARG, "expert_linear: bad shape");
+  if (rows == 0 || N == 0) return LC_OK;
+  if (positions ? x_rows * top_k != rows : x_rows != rows)
+    return fail(LC_ERR_INVALID_ARG, "expert_linear: the input's rows do not match the number of product rows");
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < lc_expert_linear_workspace_bytes(rows, K))
+    return fail(LC_ERR_WORKSPACE, "expert_linear: workspace of %lld bytes (256-byte aligned) required",
+                (long long)lc_expert_linear_workspace_bytes(rows, K));
+  uint8_t* codes = static_cast<uint8_t*>(workspace);
+  float* scale = reinterpret_cast<float*>(codes + round256(rows * pad16(K)));
+  if (int32_t rc = lc_quantize_tokens(x, x_dtype, x_rows, K, ldx, positions, top_k, rows,
+                                      offsets && !positions ? offsets + groups : nullptr,
+                                      reinterpret_cast<int8_t*>(codes), pad16(K), scale, stream))
+    return rc;
+  return grouped::check_and_launch("expert_linear", codes, 0, pad16(K), rows, offsets, groups, wq, ldw, group_stride, N,
+                                   K, scale, 1, nullptr, nullptr, sw, bias, activation, residual, ldr, out, out_dtype,
+                                   ldo, status, 0, 1, as_stream(stream));
+}

@@ -16,6 +16,9 @@ from ._loader import (LC_BF16, LC_F16, LC_F32, LC_QLINEAR_MULTICAST_OUT, LC_QLIN
 
 _dynamic_linear_f32 = entry("dynamic_linear_f32")
 _group_matmul_ex = entry("group_matmul_ex")
+_expert_linear = entry("expert_linear")
+_route_experts = entry("route_experts")
+_combine_experts = entry("combine_experts")
 _wo_linear_s8_ex = entry("wo_linear_s8_ex")
 _wo_swiglu_s8_ex = entry("wo_swiglu_s8_ex")
 
@@ -346,6 +349,109 @@ def dynamic_quantize_tensor(x2d, symmetric: bool, qmin: int, qmax: int, signed: 
                                                  _lc_dtype(out_dtype), ldq, scale.data_ptr(), zp.data_ptr(),
                                                  minmax.data_ptr(), ws.data_ptr(), ws.numel(), _stream(dev)))
     return store[:, :cols], scale, zp, minmax
+
+
+# ----------------------------------------------------------------------------
+# Linear with a fused epilogue, one or many groups; router and combination of experts
+# ----------------------------------------------------------------------------
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "swiglu": 5}
+
+
+def quantize_tokens(x2d, positions=None, out_rows: int | None = None, valid=None):
+    """Row-wise symmetric int8 codes of fp32 / bf16 / f16 rows and one scale per row, in storage whose row
+    stride is a multiple of 16 bytes.  ``positions`` [rows, copies] int32 sends token t to those rows of the
+    ``out_rows`` results (negative: nowhere; rows nothing is sent to stay uninitialised)."""
+    dev = _need_cuda(x2d, positions, valid)
+    if x2d.stride(1) != 1:
+        x2d = x2d.contiguous()
+    rows, cols = x2d.shape
+    n = rows if out_rows is None else out_rows
+    ldq = _pad16(cols)
+    store = torch.empty((n, ldq), dtype=torch.int8, device=dev)
+    scale = torch.empty(n, dtype=torch.float32, device=dev)
+    with _on(dev):
+        check(lib.lc_quantize_tokens(x2d.data_ptr(), _lc_dtype(x2d.dtype), rows, cols, x2d.stride(0), _ptr(positions),
+                                     1 if positions is None else positions.shape[1], n, _ptr(valid), store.data_ptr(),
+                                     ldq, scale.data_ptr(), _stream(dev)))
+    return store[:, :cols], scale
+
+
+def grouped_qlinear_i8(q, wq, sx, sw, bias=None, offsets=None, zx=None, wsum=None, activation: str | None = None,
+                       residual=None, out_dtype: torch.dtype = torch.float32, status=None, variant: int = 0):
+    """Product of int8 / uint8 codes ``q`` [R, K] (rows sorted by group) with the int8 weights ``wq`` [E, N, K]
+    or [N, K], scaled, with bias, activation and residual (``lc_grouped_qlinear_i8``).  ``offsets``: [E + 1]
+    int32, rows of each group; ``variant``: 0 automatic, 1 narrow tiles with K split, 2 CTA pairs."""
+    dev = _need_cuda(q, wq, sx, sw, bias, offsets, zx, wsum, residual, status)
+    if wq.dim() == 2:
+        wq = wq.unsqueeze(0)
+    groups, n, k = wq.shape
+    rows = q.shape[0]
+    width = n // 2 if activation == "swiglu" else n
+    out = torch.empty((rows, width), dtype=out_dtype, device=dev)
+    sx = _f32c(sx).reshape(-1)
+    if sx.numel() not in (1, rows):
+        raise ValueError(f"grouped_qlinear_i8: sx has {sx.numel()} entries, expected 1 or {rows}")
+    with _on(dev):
+        check(lib.lc_grouped_qlinear_i8(
+            q.data_ptr(), int(q.dtype == torch.uint8), q.stride(0), rows, _ptr(offsets), groups, wq.data_ptr(),
+            wq.stride(1), wq.stride(0), n, k, sx.data_ptr(), int(sx.numel() == rows and rows != 1), _ptr(zx), _ptr(wsum),
+            sw.data_ptr(), _ptr(bias), ACTIVATIONS[activation], _ptr(residual),
+            0 if residual is None else residual.stride(0), out.data_ptr(), _lc_dtype(out_dtype), width, _ptr(status),
+            int(variant), _stream(dev)))
+    return out
+
+
+def expert_linear(x2d, wq, sw, bias, positions, offsets, rows: int, activation: int, residual, width: int,
+                  out_dtype: torch.dtype):
+    """Row-wise quantization of ``x2d`` and the grouped product from one library call.  Arguments are taken as
+    they are (the functional layer checks them): ``wq`` [E, N, K] or [N, K] with 16-byte row pitch."""
+    dev = x2d.device
+    k = x2d.shape[1]
+    if wq.dim() == 3:
+        groups, n, ldw, stride = wq.shape[0], wq.shape[1], wq.stride(1), wq.stride(0)
+    else:
+        groups, n, ldw, stride = 1, wq.shape[0], wq.stride(0), 0
+    out = torch.empty((rows, width), dtype=out_dtype, device=dev)
+    need = (rows * _pad16(k) + 255) // 256 * 256 + (rows * 4 + 255) // 256 * 256  # lc_expert_linear_workspace_bytes
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        check(_expert_linear(x2d.data_ptr(), _DTYPE[x2d.dtype], x2d.shape[0], x2d.stride(0), _ptr(positions),
+                             1 if positions is None else positions.shape[1], _ptr(offsets), groups, rows, wq.data_ptr(),
+                             ldw, stride, n, k, sw.data_ptr(), _ptr(bias), activation, _ptr(residual),
+                             0 if residual is None else residual.stride(0), out.data_ptr(), _DTYPE[out_dtype], width,
+                             ws.data_ptr(), need, None, _stream(dev)))
+    return out
+
+
+def route_experts(logits, top_k: int, renormalize: bool):
+    """``(weights, experts, offsets, positions)`` of the router (``lc_route_experts``)."""
+    dev = _need_cuda(logits)
+    if logits.stride(1) != 1:
+        logits = logits.contiguous()
+    t, e = logits.shape
+    weights = torch.empty((t, top_k), dtype=torch.float32, device=dev)
+    experts = torch.empty((t, top_k), dtype=torch.int32, device=dev)
+    positions = torch.empty((t, top_k), dtype=torch.int32, device=dev)
+    offsets = torch.empty(e + 1, dtype=torch.int32, device=dev)
+    need = int(lib.lc_route_experts_workspace_bytes(t, e))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    with _on(dev):
+        check(_route_experts(logits.data_ptr(), _lc_dtype(logits.dtype), t, e, logits.stride(0), top_k,
+                             1 if renormalize else 0, weights.data_ptr(), experts.data_ptr(), offsets.data_ptr(),
+                             positions.data_ptr(), _ptr(ws), need, _stream(dev)))
+    return weights, experts, offsets, positions
+
+
+def combine_experts(y, weights, positions, residual=None):
+    """``sum_j weights[t, j] * y[positions[t, j]] (+ residual[t])`` (``lc_combine_experts``)."""
+    dev = _need_cuda(y, weights, positions, residual)
+    t, top_k = positions.shape
+    out = torch.empty((t, y.shape[1]), dtype=y.dtype, device=dev)
+    with _on(dev):
+        check(_combine_experts(y.data_ptr(), _DTYPE[y.dtype], y.shape[0], y.shape[1], y.stride(0), weights.data_ptr(),
+                               positions.data_ptr(), t, top_k, _ptr(residual),
+                               0 if residual is None else residual.stride(0), out.data_ptr(), y.shape[1], _stream(dev)))
+    return out
 
 
 # ----------------------------------------------------------------------------
