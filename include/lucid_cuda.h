@@ -311,8 +311,8 @@ int32_t lc_dynamic_linear_f32(const float* x, int64_t ldx, int64_t M, int64_t K,
  * activation: LC_ACT_*; with LC_ACT_SWIGLU the N weight rows are blocks of 8 gate rows and the matching 8 up
  * rows, and out and residual have N/2 columns: silu(gate) * up.  residual: of out_dtype, or NULL.
  * out_dtype LC_F32, LC_BF16 or LC_F16.  Rows of q and wq on 16-byte boundaries, K <= 65536, groups <= 1024.
- * variant: 0 automatic, 1 128 x 64 tiles with K split over a cluster, 2 256 x 256 tiles of CTA pairs, all with
- * identical results; | LC_QLINEAR_WAIT_TEST as for lc_qlinear_i8_ex.  status: see lc_qlinear_check_status. */
+ * variant: 0 automatic, 1 128 x 64 tiles with K split over a cluster, 2 256 x 256 tiles of CTA pairs, 3 .. 6 the
+ * split form with clusters of 1, 2, 4, 8 CTAs (1 where K has fewer 128-byte blocks), all with identical results; | LC_QLINEAR_WAIT_TEST as for lc_qlinear_i8_ex.  status: see lc_qlinear_check_status. */
 #define LC_ACT_NONE 0
 #define LC_ACT_RELU 1
 #define LC_ACT_GELU 2      /* 0.5 v (1 + erf(v / sqrt 2)) */

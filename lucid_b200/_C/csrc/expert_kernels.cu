@@ -100,7 +100,7 @@ __device__ __forceinline__ int block_scan(int v, int* tmp) {
 }
 
 template <typename T, int EPL, bool ONE_CTA>
-__global__ void __launch_bounds__(ONE_CTA ? 1024 : 256) route_kernel(const RouteParams p) {
+__global__ void __launch_bounds__(1024) route_kernel(const RouteParams p) {
   extern __shared__ int s_counts[];  // [warps][experts]; one CTA: then [experts] bases
   __shared__ int s_tmp[32];
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -201,72 +201,87 @@ __global__ void __launch_bounds__(ONE_CTA ? 1024 : 256) route_kernel(const Route
 }
 
 // second kernel of a large batch: CTA b adds to its tokens' ranks the rows of the experts before and the
-// counts of the CTAs before it
-__global__ void __launch_bounds__(256) route_place_kernel(const RouteParams p, int ctas, int64_t tokens_per_cta) {
-  __shared__ int s_base[kRouteMaxExperts];
+// counts of the CTAs before it.  1024 / (experts rounded up to a power of two, at least 32) groups of threads
+// share the CTAs' counts, one column each.
+__global__ void __launch_bounds__(1024) route_place_kernel(const RouteParams p, int ctas, int64_t tokens_per_cta,
+                                                           int width_log2) {
+  __shared__ int s_sum[1024], s_before[1024];
   __shared__ int s_tmp[32];
   pdl_launch_dependents();
   pdl_wait();
-  const int E = p.experts;
-  int carry = 0;
-  for (int e0 = 0; e0 < E; e0 += 256) {
-    const int e = e0 + threadIdx.x;
-    int before = 0, sum = 0;
-    if (e < E) {
-      const int32_t* c = p.counts + e;
+  const int E = p.experts, width = 1 << width_log2, parts = 1024 >> width_log2;
+  const int e = threadIdx.x & (width - 1), part = threadIdx.x >> width_log2;
+  int before = 0, sum = 0;
+  if (e < E) {
+    const int32_t* c = p.counts + e;
 #pragma unroll 8
-      for (int b = 0; b < ctas; ++b) {
-        const int v = __ldg(c + static_cast<int64_t>(b) * E);
-        if (b < static_cast<int>(blockIdx.x)) before += v;
-        sum += v;
-      }
+    for (int b = part; b < ctas; b += parts) {
+      const int v = __ldg(c + static_cast<int64_t>(b) * E);
+      if (b < static_cast<int>(blockIdx.x)) before += v;
+      sum += v;
     }
-    const int end = block_scan(sum, s_tmp);
-    if (e < E) {
-      s_base[e] = carry + end - sum + before;
-      if (blockIdx.x == 0) {
-        p.offsets[e + 1] = carry + end;
-        if (e == 0) p.offsets[0] = 0;
-      }
+  }
+  s_sum[threadIdx.x] = sum;
+  s_before[threadIdx.x] = before;
+  __syncthreads();
+  sum = before = 0;
+  if (static_cast<int>(threadIdx.x) < width)
+    for (int i = 0; i < parts; ++i) {
+      sum += s_sum[(i << width_log2) + e];
+      before += s_before[(i << width_log2) + e];
     }
-    carry += s_tmp[7];
+  const int end = block_scan(sum, s_tmp);
+  if (static_cast<int>(threadIdx.x) < E) {
+    s_before[threadIdx.x] = end - sum + before;
+    if (blockIdx.x == 0) {
+      p.offsets[e + 1] = end;
+      if (e == 0) p.offsets[0] = 0;
+    }
   }
   __syncthreads();
   const int64_t first = blockIdx.x * tokens_per_cta;
   const int64_t last = first + tokens_per_cta < p.tokens ? first + tokens_per_cta : p.tokens;
-  for (int64_t i = first * p.top_k + threadIdx.x; i < last * p.top_k; i += 256) {
-    const int e = p.chosen[i];
-    if (e >= 0) p.positions[i] += s_base[e];
+  for (int64_t i = first * p.top_k + threadIdx.x; i < last * p.top_k; i += 1024) {
+    const int at = p.chosen[i];
+    if (at >= 0) p.positions[i] += s_before[at];
   }
 }
 
-constexpr int64_t kRouteOneCta = 128;  // tokens
-constexpr int kRouteRun = 16;          // tokens per warp of a large batch
-constexpr int64_t kRouteWarps = 8;
+constexpr int kRouteWarps = 32;
+constexpr int64_t kRouteOneCta = 128;  // tokens that one CTA routes and places in one kernel
+constexpr int64_t kRouteCtas = 128;    // CTAs of a larger batch: tokens per warp grow beyond that
+
+int64_t route_run(int64_t tokens) {  // tokens per warp
+  return (tokens + kRouteCtas * kRouteWarps - 1) / (kRouteCtas * kRouteWarps);
+}
 
 template <typename T, int EPL>
 cudaError_t launch_route(RouteParams p, cudaStream_t st) {
-  if (p.tokens <= kRouteOneCta) {
-    p.run = static_cast<int>((p.tokens + 31) / 32);
-    const size_t smem = static_cast<size_t>(33) * p.experts * 4;
-    static std::once_flag flags[64];
-    static cudaError_t results[64];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    std::call_once(flags[dev], [dev]() {
-      results[dev] = cudaFuncSetAttribute(route_kernel<T, EPL, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          33 * EPL * 32 * 4);
-    });
-    if (results[dev] != cudaSuccess) return results[dev];
+  static std::once_flag flags[64][2];
+  static cudaError_t results[64][2];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  const int one = p.tokens <= kRouteOneCta;
+  std::call_once(flags[dev][one], [dev, one]() {
+    const int bytes = (kRouteWarps + 1) * EPL * 32 * 4;
+    results[dev][one] =
+        one ? cudaFuncSetAttribute(route_kernel<T, EPL, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)
+            : cudaFuncSetAttribute(route_kernel<T, EPL, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  });
+  if (results[dev][one] != cudaSuccess) return results[dev][one];
+  const size_t smem = static_cast<size_t>(kRouteWarps + 1) * p.experts * 4;
+  if (one) {
+    p.run = static_cast<int>((p.tokens + kRouteWarps - 1) / kRouteWarps);
     return launch_overlapped(route_kernel<T, EPL, true>, dim3(1), dim3(1024), smem, st, p);
   }
-  p.run = kRouteRun;
-  const int64_t per_cta = kRouteWarps * p.run;
+  p.run = static_cast<int>(route_run(p.tokens));
+  const int64_t per_cta = static_cast<int64_t>(kRouteWarps) * p.run;
   const int ctas = static_cast<int>((p.tokens + per_cta - 1) / per_cta);
-  cudaError_t err = launch_overlapped(route_kernel<T, EPL, false>, dim3(ctas), dim3(256),
-                                      static_cast<size_t>(kRouteWarps) * p.experts * 4, st, p);
+  cudaError_t err = launch_overlapped(route_kernel<T, EPL, false>, dim3(ctas), dim3(1024), smem, st, p);
   if (err != cudaSuccess) return err;
-  return launch_overlapped(route_place_kernel, dim3(ctas), dim3(256), 0, st, p, ctas, per_cta);
+  int width_log2 = 5;
+  while ((1 << width_log2) < p.experts) ++width_log2;
+  return launch_overlapped(route_place_kernel, dim3(ctas), dim3(1024), 0, st, p, ctas, per_cta, width_log2);
 }
 
 template <typename T>
@@ -301,6 +316,21 @@ struct TokenParams {
   float* scale;
 };
 
+// largest |x| of 16 bytes (fmaxf and __hmax2 drop NaN); 16-bit types two at a time
+__device__ __forceinline__ float largest_of(const Vec16<float>& v) {
+  return fmaxf(fmaxf(fabsf(v.v[0]), fabsf(v.v[1])), fmaxf(fabsf(v.v[2]), fabsf(v.v[3])));
+}
+template <typename T, typename T2>
+__device__ __forceinline__ float largest_of_pairs(const T* v) {
+  const T2* w = reinterpret_cast<const T2*>(v);
+  const T2 m = __hmax2(__hmax2(__habs2(w[0]), __habs2(w[1])), __hmax2(__habs2(w[2]), __habs2(w[3])));
+  return fmaxf(to_float<T>(m.x), to_float<T>(m.y));
+}
+__device__ __forceinline__ float largest_of(const Vec16<__nv_bfloat16>& v) {
+  return largest_of_pairs<__nv_bfloat16, __nv_bfloat162>(v.v);
+}
+__device__ __forceinline__ float largest_of(const Vec16<__half>& v) { return largest_of_pairs<__half, __half2>(v.v); }
+
 __device__ __forceinline__ float token_scale(float largest) { return fmaxf(__fdiv_rn(largest, 127.5f), 1e-8f); }
 
 // TPR threads hold a row of up to TPR * ITEMS vectors; 256 / TPR rows (at least one) per CTA
@@ -324,10 +354,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) quantize_tokens_kernel(
   }
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
-    if (live && i * TPR + sub < vectors) {
-#pragma unroll
-      for (int j = 0; j < VN; ++j) largest = fmaxf(largest, fabsf(to_float<T>(v[i].v[j])));  // (fmaxf drops NaN)
-    }
+    if (live && i * TPR + sub < vectors) largest = fmaxf(largest, largest_of(v[i]));
   }
   largest = warp_max(largest);
   if (TPR > 32) {
@@ -406,6 +433,7 @@ cudaError_t launch_tokens(const TokenParams& p, cudaStream_t st) {
   if (vectors <= 32) return launch_overlapped(quantize_tokens_kernel<T, 32, 1>, grid(8), dim3(256), 0, st, p);
   if (vectors <= 128) return launch_overlapped(quantize_tokens_kernel<T, 32, 4>, grid(8), dim3(256), 0, st, p);
   if (vectors <= 512) return launch_overlapped(quantize_tokens_kernel<T, 128, 4>, grid(2), dim3(256), 0, st, p);
+  if (vectors <= 1024) return launch_overlapped(quantize_tokens_kernel<T, 256, 4>, grid(1), dim3(256), 0, st, p);
   if (vectors <= 2048) return launch_overlapped(quantize_tokens_kernel<T, 512, 4>, grid(1), dim3(512), 0, st, p);
   return launch_overlapped(quantize_tokens_kernel<T, 512, 8>, grid(1), dim3(512), 0, st, p);
 }
@@ -514,7 +542,7 @@ using namespace lc;
 
 extern "C" int64_t lc_route_experts_workspace_bytes(int64_t tokens, int64_t experts) {
   if (tokens <= kRouteOneCta || experts <= 0) return 0;
-  const int64_t per_cta = kRouteWarps * kRouteRun;
+  const int64_t per_cta = kRouteWarps * route_run(tokens);
   return (tokens + per_cta - 1) / per_cta * experts * 4;
 }
 

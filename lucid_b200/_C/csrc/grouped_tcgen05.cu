@@ -55,7 +55,6 @@ struct Cfg<2> {
   static constexpr int kBox = 32;     // q rows per TMA box
   static constexpr int kStages = 6;
   static constexpr int kBBytes = (kTokens / 2) * BK;
-  static constexpr int kChunk = 32;   // accumulator columns an epilogue warp takes at a time
   static constexpr int kRedBytes = 0;
 };
 template <>
@@ -66,7 +65,6 @@ struct Cfg<1> {
   static constexpr int kBox = 16;
   static constexpr int kStages = 7;
   static constexpr int kBBytes = kTokens * BK;
-  static constexpr int kChunk = 16;
   static constexpr int kRedBytes = kTokens * WROWS * 4;  // partial sums of the other ranks, [column][lane]
 };
 template <int CG>
@@ -148,7 +146,6 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(cluster_bar)
       : "memory");
 }
-__device__ __forceinline__ void tc_ld(uint32_t taddr, uint32_t (&r)[32]) { tc_ld_32x32(taddr, r); }
 __device__ __forceinline__ void tc_ld(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -208,24 +205,44 @@ struct TileWalk {
 };
 
 // ---- epilogue arithmetic -------------------------------------------------------------------
-// EXACT for fp32 results (library expf and IEEE division); 16-bit results take the hardware exponential and
-// the approximate division, whose relative errors (below 2^-20 for the arguments that matter) vanish in the
-// rounding to 8 or 11 bits.
-template <bool EXACT>
-__device__ __forceinline__ float sigmoid_times(float v, float arg) {  // v / (1 + exp(-arg))
-  if (EXACT) return __fdiv_rn(v, 1.0f + expf(-arg));
-  return __fdividef(v, 1.0f + __expf(-arg));
+// Sigmoids take the hardware exponential and the approximate division: with z = -arg, ex2's argument carries a
+// relative rounding of 2^-23, so exp(z) is off by (2 + 1.2 |z|) 2^-23, which sigma (1 - sigma) turns into less than
+// 2^-23 of v, next to the division's 2 ulp.
+__device__ __forceinline__ float sigmoid_times(float v, float arg) { return __fdividef(v, 1.0f + __expf(-arg)); }
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
-template <bool EXACT>
-__device__ __forceinline__ float activate(float v, int act) {
-  switch (act) {
-    case LC_ACT_RELU: return v < 0.0f ? 0.0f : v;  // NaN compares false and stays
-    case LC_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678118654752440f));
-    case LC_ACT_GELU_TANH:  // 0.5 v (1 + tanh(u)) = v / (1 + exp(-2u)), u = sqrt(2/pi) (v + 0.044715 v^3)
-      return sigmoid_times<EXACT>(v, 1.5957691216057307f * (v + 0.044715f * v * v * v));
-    case LC_ACT_SILU: return sigmoid_times<EXACT>(v, v);
-    default: return v;
-  }
+// v * Phi(v), Phi the normal distribution function.  Phi(-a) = 2^p(a) for a = |v|, p a polynomial of degree 9 fitted
+// to log2 Phi(-a) on [0, 6] (least squares over Chebyshev nodes, reweighted towards the smallest largest error in
+// a * Phi): a * Phi(-a) is off by at most 3.5e-8, and by 2e-12 beyond 6.  15 instructions where the library's erff
+// takes about 40: on an 8192 x 2048 x 512 product, whose time is the epilogue's, 45 us against TODO us.
+__device__ __forceinline__ float gelu(float v) {
+  const float a = fminf(fabsf(v), 10.0f);
+  float p = 2.9685912750210264e-07f;
+  p = fmaf(p, a, -6.425118044717237e-06f);
+  p = fmaf(p, a, 5.635188063024543e-05f);
+  p = fmaf(p, a, -0.00022571126464754343f);
+  p = fmaf(p, a, -9.095141285797581e-05f);
+  p = fmaf(p, a, 0.007042091339826584f);
+  p = fmaf(p, a, -0.052499450743198395f);
+  p = fmaf(p, a, -0.4592026472091675f);
+  p = fmaf(p, a, -1.151106357574463f);
+  p = fmaf(p, a, -0.9999999403953552f);
+  const float t = exp2_approx(p);
+  return v * (v > 0.0f ? 1.0f - t : t);
+}
+
+template <int ACT>
+__device__ __forceinline__ float activate(float v) {
+  if constexpr (ACT == LC_ACT_RELU) return v < 0.0f ? 0.0f : v;  // NaN compares false and stays
+  if constexpr (ACT == LC_ACT_GELU) return gelu(v);
+  if constexpr (ACT == LC_ACT_GELU_TANH)  // 0.5 v (1 + tanh(u)) = v / (1 + exp(-2u)), u = sqrt(2/pi) (v + 0.044715 v^3)
+    return sigmoid_times(v, 1.5957691216057307f * (v + 0.044715f * v * v * v));
+  if constexpr (ACT == LC_ACT_SILU) return sigmoid_times(v, v);
+  return v;
 }
 
 template <typename T>
@@ -245,76 +262,94 @@ __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return
 template <>
 __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
 
-// One chunk of CH accumulator columns: this lane's output column `n` of the rows row0 .. row0 + rows - 1.
-template <typename T, int CH>
-__device__ __forceinline__ void finish_chunk(const Params& p, const uint32_t (&r)[CH], int64_t row0, int rows,
-                                             int64_t n, int lane, const float* sx, float sw, float bias, int corr) {
-  constexpr bool kExact = sizeof(T) == 4;
-  float f[CH];
+// What an epilogue warp knows of its tile: its lane's weight row and the columns it drains.
+struct Lane {
+  uint32_t t_row;   // TMEM address of this warp's quadrant of the accumulator
+  int64_t m0;       // first row of q
+  int rows;
+  int64_t n;        // this lane's weight row inside the group
+  float sw, bias;
+  int corr;         // zx * wsum
+  const float* sx;  // scales of the tile's rows
+  int first;        // first column this warp takes; every second chunk from there
+  int slot;         // this lane's word in a row of the partial-sum buffer
+  int* red;         // rank 0 of a split tile: the other ranks' sums, cleared as they are read; else null
+};
+
+// Drains the accumulator in chunks of 16 columns: 16 rows of q, 32 adjacent outputs of each per warp.  The
+// activation and the type are compiled in and the loop over the chunks is not unrolled: with all of them in one
+// unrolled body (5000 instructions and more) the epilogue ran at the speed of instruction fetch, 30 us per
+// 256 x 256 tile.
+constexpr int CH = 16;
+template <typename T, int ACT>
+__device__ __forceinline__ void drain(const Params& p, const Lane& l) {
+  const bool in = l.n < p.N;
+  const int up = (static_cast<int>(l.n) >> 3) & 1;  // SwiGLU: this lane's weight row is an up row
+  const int64_t col = ACT == LC_ACT_SWIGLU ? (((l.n >> 4) << 3) | (l.n & 7)) : l.n;
+  const int64_t row0 = l.m0 + (ACT == LC_ACT_SWIGLU ? up : 0);
+  const T* const res = static_cast<const T*>(p.residual);
+#pragma unroll 1
+  for (int c = l.first; c < l.rows; c += 2 * CH) {
+    uint32_t r[CH];
+    tc_ld(l.t_row + static_cast<uint32_t>(c), r);
+    const int left = in ? l.rows - c : 0;
+    constexpr int kStep = ACT == LC_ACT_SWIGLU ? 2 : 1;  // a lane finishes every row, or every second one
+    T rv[CH / kStep];
+    if (res) {
+      const T* src = res + (row0 + c) * p.ldr + col;
 #pragma unroll
-  for (int j = 0; j < CH; j += 4) {
-    const float4 s = *reinterpret_cast<const float4*>(sx + j);
-    const float sv[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      f[j + i] = __fadd_rn(__fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(r[j + i]) - corr), sv[i]), sw), bias);
-  }
-  if (p.act == LC_ACT_SWIGLU) {
-    // lanes 8 apart hold the gate and up value of one unit: each finishes every other row
-    const int up = (lane >> 3) & 1;
-    const int64_t unit = ((n >> 4) << 3) | (n & 7);
-    T* o = static_cast<T*>(p.out) + (row0 + up) * p.ldo + unit;
-    const T* res = static_cast<const T*>(p.residual) + (p.residual ? (row0 + up) * p.ldr + unit : 0);
-#pragma unroll
-    for (int j = 0; j < CH; j += 2) {
-      const float got = __shfl_xor_sync(0xffffffffu, up ? f[j] : f[j + 1], 8);
-      const float gate = up ? got : f[j], lin = up ? f[j + 1] : got;
-      float v = sigmoid_times<kExact>(gate, gate) * lin;
-      if (j + up < rows && n < p.N) {
-        if (p.residual) v += widen<T>(res[j * p.ldr]);
-        o[j * p.ldo] = narrow<T>(v);
+      for (int j = 0; j < CH; j += kStep) {
+        if (j + (kStep == 2 ? up : 0) < left) rv[j / kStep] = *src;
+        src += kStep * p.ldr;
       }
     }
-    return;
+    tc_wait_ld();
+    if (l.red) {
+      int* mine = l.red + c * WROWS + l.slot;
+#pragma unroll
+      for (int j = 0; j < CH; ++j) {
+        if (c + j < l.rows) {
+          r[j] += static_cast<uint32_t>(mine[j * WROWS]);
+          mine[j * WROWS] = 0;
+        }
+      }
+    }
+    float f[CH];
+#pragma unroll
+    for (int j = 0; j < CH; j += 4) {
+      const float4 s = *reinterpret_cast<const float4*>(l.sx + c + j);
+      const float sv[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        f[j + i] = __fadd_rn(__fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(r[j + i]) - l.corr), sv[i]), l.sw), l.bias);
+    }
+    T* o = static_cast<T*>(p.out) + (row0 + c) * p.ldo + col;
+#pragma unroll
+    for (int j = 0; j < CH; j += kStep) {
+      float v;
+      if constexpr (ACT == LC_ACT_SWIGLU) {
+        // lanes 8 apart hold the gate and the up value of one unit: each finishes every other row
+        const float got = __shfl_xor_sync(0xffffffffu, up ? f[j] : f[j + 1], 8);
+        const float gate = up ? got : f[j], lin = up ? f[j + 1] : got;
+        v = sigmoid_times(gate, gate) * lin;
+      } else {
+        v = activate<ACT>(f[j]);
+      }
+      if (j + (kStep == 2 ? up : 0) < left) {
+        if (res) v += widen<T>(rv[j / kStep]);
+        *o = narrow<T>(v);
+      }
+      o += kStep * p.ldo;
+    }
   }
-  if (p.act != LC_ACT_NONE) {
-#pragma unroll
-    for (int j = 0; j < CH; ++j) f[j] = activate<kExact>(f[j], p.act);
-  }
-  if (n >= p.N) return;
-  if (p.residual) {
-    const T* res = static_cast<const T*>(p.residual) + row0 * p.ldr + n;
-    T v[CH];
-#pragma unroll
-    for (int j = 0; j < CH; ++j)
-      if (j < rows) v[j] = res[j * p.ldr];
-#pragma unroll
-    for (int j = 0; j < CH; ++j)
-      if (j < rows) f[j] += widen<T>(v[j]);
-  }
-  T* o = static_cast<T*>(p.out) + row0 * p.ldo + n;
-#pragma unroll
-  for (int j = 0; j < CH; ++j)
-    if (j < rows) o[j * p.ldo] = narrow<T>(f[j]);
 }
 
-template <int CH>
-__device__ __forceinline__ void finish(const Params& p, const uint32_t (&r)[CH], int64_t row0, int rows, int64_t n,
-                                       int lane, const float* sx, float sw, float bias, int corr) {
-  if (p.out_dtype == LC_F32)
-    finish_chunk<float, CH>(p, r, row0, rows, n, lane, sx, sw, bias, corr);
-  else if (p.out_dtype == LC_BF16)
-    finish_chunk<__nv_bfloat16, CH>(p, r, row0, rows, n, lane, sx, sw, bias, corr);
-  else
-    finish_chunk<__half, CH>(p, r, row0, rows, n, lane, sx, sw, bias, corr);
-}
-
-template <int CG>
+template <int CG, typename T, int ACT>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_q,
-                      const Params p) {
+                      const __grid_constant__ CUtensorMap tmap_q_full, const Params p) {
   using C = Cfg<CG>;
-  constexpr int STAGES = C::kStages, STAGE_BYTES = stage_bytes<CG>(), CH = C::kChunk;
+  constexpr int STAGES = C::kStages, STAGE_BYTES = stage_bytes<CG>();
   constexpr int TMEM_COLS = 2 * C::kTokens;  // 512 or 128
   static_assert(2 * STAGES * 8 + 6 * 8 <= 256, "barrier area");
   extern __shared__ uint8_t smem_raw[];
@@ -420,9 +455,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   if (warp == 0) {
     // ===================== TMA producer =====================
     if (lane == 0) {
-      uint32_t armed_parity[STAGES];
-      bool armed[STAGES];
-      for (int s = 0; s < STAGES; ++s) armed[s] = false;
+      uint32_t armed = 0, armed_parity = 0;  // one bit per stage
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true, waited = !p.early_weights;
@@ -435,10 +468,11 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         const uint32_t bytes = CG * (A_BYTES + boxes * C::kBox * BK);
         const int n0 = static_cast<int>(tile.n0) + (CG == 2 ? static_cast<int>(rank) * WROWS : 0);
         const int m0 = tile.m0 + (CG == 2 ? static_cast<int>(rank) * mine : 0);
-        auto arm = [&](int s) {
+        auto arm = [&](int s, uint32_t parity) {
           if (CG == 1 || leader) {
             mbar_expect_tx(full_bar(s), bytes);
-            armed[s] = true;
+            armed |= 1u << s;
+            armed_parity = (armed_parity & ~(1u << s)) | (parity << s);
           }
         };
         auto load_w = [&](int s, int kb) {
@@ -450,6 +484,13 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         };
         auto load_q = [&](int s, int kb) {
           const uint32_t dst = tiles_base + s * STAGE_BYTES + A_BYTES;
+          if (mine == C::kTokens / CG) {  // a full tile: one box instead of four
+            if constexpr (CG == 2)
+              tma_load_2d_pair(dst, &tmap_q_full, kb * BK, m0, map_to_cta(full_bar(s), 0));
+            else
+              tma_load_2d(dst, &tmap_q_full, kb * BK, m0, full_bar(s));
+            return;
+          }
           for (int b = 0; b < boxes; ++b) {
             if constexpr (CG == 2)
               tma_load_2d_pair(dst + b * C::kBox * BK, &tmap_q, kb * BK, m0 + b * C::kBox, map_to_cta(full_bar(s), 0));
@@ -462,8 +503,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
           // the ring is empty: fill it with weights while the kernel before this one still writes the codes
           const int ahead = min(STAGES, kb1 - kb0);
           for (int s = 0; s < ahead; ++s) {
-            arm(s);
-            armed_parity[s] = 0;
+            arm(s, 0);
             load_w(s, kb0 + s);
           }
           pdl_wait();
@@ -479,8 +519,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
             ok = false;
             break;
           }
-          arm(stage);
-          armed_parity[stage] = phase;
+          arm(stage, phase);
           load_w(stage, kb);
           load_q(stage, kb);
           if (++stage == STAGES) {
@@ -491,7 +530,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       }
       // do not leave while a bulk copy may still be landing (a pair's leader counts the bytes of both CTAs)
       for (int s = 0; s < STAGES; ++s)
-        if (armed[s]) mbar_wait(full_bar(s), armed_parity[s]);
+        if (armed >> s & 1) mbar_wait(full_bar(s), armed_parity >> s & 1);
     }
   } else if (warp == 1) {
     // ===================== MMA issuer (a pair's leader only) =====================
@@ -576,32 +615,31 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         break;
       }
       tc_fence_after();
-      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(as * C::kTokens);
+      Lane l;
+      l.t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(as * C::kTokens);
+      l.m0 = tile.m0;
+      l.rows = tile.rows;
+      l.n = n;
+      l.sw = sw;
+      l.bias = bias;
+      l.corr = corr;
+      l.sx = sx;
+      l.first = group * CH;
+      l.slot = q * 32 + lane;
+      l.red = CG == 1 && p.split > 1 ? s_red : nullptr;
+      if (CG == 1 && !leader) {
+        const uint32_t dst = map_to_cta(red_base, 0) + static_cast<uint32_t>(l.slot) * 4;
 #pragma unroll 1
-      for (int c = group * CH; c < tile.rows; c += 2 * CH) {
-        uint32_t r[CH];
-        tc_ld(t_row + static_cast<uint32_t>(c), r);
-        tc_wait_ld();
-        if (CG == 1 && p.split > 1) {
-          const uint32_t slot = static_cast<uint32_t>((c * WROWS + q * 32 + lane) * 4);
-          if (!leader) {
-            const uint32_t dst = map_to_cta(red_base, 0) + slot;
+        for (int c = l.first; c < l.rows; c += 2 * CH) {
+          uint32_t r[CH];
+          tc_ld(l.t_row + static_cast<uint32_t>(c), r);
+          tc_wait_ld();
 #pragma unroll
-            for (int j = 0; j < CH; ++j)
-              if (c + j < tile.rows) red_add_cluster(dst + j * WROWS * 4, r[j]);
-            continue;
-          }
-          int* const mine = s_red + slot / 4;
-#pragma unroll
-          for (int j = 0; j < CH; ++j) {
-            if (c + j < tile.rows) {
-              r[j] += static_cast<uint32_t>(mine[j * WROWS]);
-              mine[j * WROWS] = 0;
-            }
-          }
+          for (int j = 0; j < CH; ++j)
+            if (c + j < l.rows) red_add_cluster(dst + static_cast<uint32_t>((c + j) * WROWS * 4), r[j]);
         }
-        const int left = tile.rows - c;
-        finish<CH>(p, r, tile.m0 + c, left < CH ? left : CH, n, lane, sx + c, sw, bias, corr);
+      } else {
+        drain<T, ACT>(p, l);
       }
       tc_fence_before();
       if (CG == 1 && p.split > 1) {
@@ -623,14 +661,9 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     }
     // rows behind the last group belong to no group: zero
     if (p.offsets) {
-      const int64_t width = p.act == LC_ACT_SWIGLU ? p.N / 2 : p.N;
+      const int64_t width = ACT == LC_ACT_SWIGLU ? p.N / 2 : p.N;
       for (int64_t row = s_off[p.E] + static_cast<int64_t>(blockIdx.x); row < p.R; row += gridDim.x)
-        for (int64_t c = et; c < width; c += EPI_THREADS) {
-          if (p.out_dtype == LC_F32)
-            static_cast<float*>(p.out)[row * p.ldo + c] = 0.0f;
-          else
-            static_cast<uint16_t*>(p.out)[row * p.ldo + c] = 0;
-        }
+        for (int64_t c = et; c < width; c += EPI_THREADS) static_cast<T*>(p.out)[row * p.ldo + c] = narrow<T>(0.0f);
     }
   }
 
@@ -652,13 +685,28 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
 }
 
 // ---- host side -------------------------------------------------------------------------------
-struct DeviceInfo {
-  cudaError_t err;
-  int clusters[4];  // resident clusters of 1, 2, 4, 8 CTAs of the split form
-};
+using Kernel = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, Params);
 
-static cudaError_t launch_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attrs, unsigned grid, int smem,
-                                 int cluster, cudaStream_t st) {
+template <int CG, typename T>
+static Kernel kernel_for(int act) {
+  switch (act) {
+    case LC_ACT_RELU: return grouped_linear_kernel<CG, T, LC_ACT_RELU>;
+    case LC_ACT_GELU: return grouped_linear_kernel<CG, T, LC_ACT_GELU>;
+    case LC_ACT_GELU_TANH: return grouped_linear_kernel<CG, T, LC_ACT_GELU_TANH>;
+    case LC_ACT_SILU: return grouped_linear_kernel<CG, T, LC_ACT_SILU>;
+    case LC_ACT_SWIGLU: return grouped_linear_kernel<CG, T, LC_ACT_SWIGLU>;
+    default: return grouped_linear_kernel<CG, T, LC_ACT_NONE>;
+  }
+}
+template <int CG>
+static Kernel kernel_for(int dtype, int act) {
+  return dtype == LC_F32    ? kernel_for<CG, float>(act)
+         : dtype == LC_BF16 ? kernel_for<CG, __nv_bfloat16>(act)
+                            : kernel_for<CG, __half>(act);
+}
+
+static void launch_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attrs, unsigned grid, int smem, int cluster,
+                          cudaStream_t st) {
   *cfg = {};
   cfg->gridDim = dim3(grid);
   cfg->blockDim = dim3(NUM_THREADS);
@@ -672,8 +720,12 @@ static cudaError_t launch_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* a
   attrs[1].val.programmaticStreamSerializationAllowed = 1;
   cfg->attrs = attrs;
   cfg->numAttrs = 2;
-  return cudaSuccess;
 }
+
+struct DeviceInfo {
+  cudaError_t err;
+  int clusters[4];  // resident clusters of 1, 2, 4, 8 CTAs of the split form
+};
 
 static int32_t device_info(const DeviceInfo** out) {
   constexpr int kMaxDevices = 64;
@@ -684,9 +736,13 @@ static int32_t device_info(const DeviceInfo** out) {
     return fail(LC_ERR_CUDA, "no current CUDA device");
   std::call_once(flags[dev], [dev]() {
     DeviceInfo& info = infos[dev];
-    info.err = cudaFuncSetAttribute(grouped_linear_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<1>());
-    if (info.err == cudaSuccess)
-      info.err = cudaFuncSetAttribute(grouped_linear_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<2>());
+    info.err = cudaSuccess;
+    for (int dtype : {LC_F32, LC_BF16, LC_F16})
+      for (int act = LC_ACT_NONE; act <= LC_ACT_SWIGLU && info.err == cudaSuccess; ++act) {
+        info.err = cudaFuncSetAttribute(kernel_for<1>(dtype, act), cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<1>());
+        if (info.err == cudaSuccess)
+          info.err = cudaFuncSetAttribute(kernel_for<2>(dtype, act), cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<2>());
+      }
     const int sms = sm_count();
     for (int i = 0; i < 4 && info.err == cudaSuccess; ++i) {
       cudaLaunchConfig_t cfg;
@@ -694,7 +750,7 @@ static int32_t device_info(const DeviceInfo** out) {
       launch_config(&cfg, attrs, static_cast<unsigned>(sms / (1 << i) << i), smem_bytes<1>(), 1 << i, nullptr);
       cfg.numAttrs = 1;
       int n = 0;
-      if (cudaOccupancyMaxActiveClusters(&n, grouped_linear_kernel<1>, &cfg) != cudaSuccess) {
+      if (cudaOccupancyMaxActiveClusters(&n, kernel_for<1>(LC_F32, LC_ACT_NONE), &cfg) != cudaSuccess) {
         cudaGetLastError();
         n = i == 0 ? sms : 0;
       }
@@ -716,12 +772,16 @@ static int32_t launch(const void* q, int64_t ldq, const int8_t* w, int64_t ldw, 
   if (int32_t rc = device_info(&info)) return rc;
   const int64_t sms = sm_count();
   const bool pair = variant == 2 || (variant == 0 && p.R > kPairRows * p.E);
-  CUtensorMap map_w, map_q;
+  const int forced = variant > 2 ? 1 << (variant - 3) : 0;
+  CUtensorMap map_w, map_q, map_q_full;
   if (int32_t rc = encode_tensor_map_3d(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, p.K, p.N, p.E, ldw, group_stride, BK,
                                         WROWS, CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
   if (int32_t rc = encode_tensor_map_2d(&map_q, CU_TENSOR_MAP_DATA_TYPE_UINT8, q, p.K, p.R, ldq, BK,
                                         pair ? Cfg<2>::kBox : Cfg<1>::kBox, CU_TENSOR_MAP_SWIZZLE_128B))
+    return rc;
+  if (int32_t rc = encode_tensor_map_2d(&map_q_full, CU_TENSOR_MAP_DATA_TYPE_UINT8, q, p.K, p.R, ldq, BK,
+                                        pair ? Cfg<2>::kTokens / 2 : Cfg<1>::kTokens, CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
   // kind::i8: D s32 (2) in bits [4,6); A (weight, s8 = 1) in [7,10), B (codes, s8 = 1 or u8 = 0) in [10,13); both
   // K-major; N >> 3 in [17,23) is filled in per tile; M >> 4 in [24,29)
@@ -742,12 +802,13 @@ static int32_t launch(const void* q, int64_t ldq, const int8_t* w, int64_t ldw, 
     const int num_kb = static_cast<int>((p.K + BK - 1) / BK);
     double best = 0.0;
     cluster = 1;
+    units = sms;
     for (int i = 0; i < 4; ++i) {
       const int s = 1 << i;
-      if (info->clusters[i] < 1 || num_kb < 4 * s) break;
+      if (info->clusters[i] < 1 || num_kb < (forced ? 1 : 4) * s) break;
       const int64_t waves = (tiles + info->clusters[i] - 1) / info->clusters[i];
       const double cost = static_cast<double>(waves) * ((num_kb + s - 1) / s + (s > 1 ? 2 : 0));
-      if (i == 0 || cost < best) {
+      if (forced ? s == forced : i == 0 || cost < best) {
         best = cost;
         cluster = s;
         units = info->clusters[i];
@@ -759,8 +820,8 @@ static int32_t launch(const void* q, int64_t ldq, const int8_t* w, int64_t ldw, 
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attrs[2];
   launch_config(&cfg, attrs, static_cast<unsigned>(units * cluster), pair ? smem_bytes<2>() : smem_bytes<1>(), cluster, st);
-  const cudaError_t err = pair ? cudaLaunchKernelEx(&cfg, grouped_linear_kernel<2>, map_w, map_q, p)
-                               : cudaLaunchKernelEx(&cfg, grouped_linear_kernel<1>, map_w, map_q, p);
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, pair ? kernel_for<2>(p.out_dtype, p.act) : kernel_for<1>(p.out_dtype, p.act),
+                                             map_w, map_q, map_q_full, p);
   if (err != cudaSuccess) return fail(LC_ERR_CUDA, "grouped_linear: %s", cudaGetErrorString(err));
   return check_launch("grouped_linear");
 }
@@ -774,7 +835,7 @@ static int32_t check_and_launch(const char* what, const void* q, int q_unsigned,
   const int wait_test = (variant & LC_QLINEAR_WAIT_TEST) ? 1 : 0;
   variant &= ~LC_QLINEAR_WAIT_TEST;
   if (wait_test && !status) return fail(LC_ERR_INVALID_ARG, "%s: the wait test needs a status word", what);
-  if (variant < 0 || variant > 2) return fail(LC_ERR_INVALID_ARG, "%s: variant must be 0, 1 or 2", what);
+  if (variant < 0 || variant > 6) return fail(LC_ERR_INVALID_ARG, "%s: variant must be between 0 and 6", what);
   if (R < 0 || N < 0 || K <= 0 || E < 1) return fail(LC_ERR_INVALID_ARG, "%s: bad shape", what);
   if (act < LC_ACT_NONE || act > LC_ACT_SWIGLU) return fail(LC_ERR_INVALID_ARG, "%s: unknown activation %d", what, act);
   if (act == LC_ACT_SWIGLU && N % 16)

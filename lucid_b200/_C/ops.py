@@ -401,31 +401,52 @@ def grouped_qlinear_i8(q, wq, sx, sw, bias=None, offsets=None, zx=None, wsum=Non
     return out
 
 
-def expert_linear(x2d, wq, sw, bias, positions, offsets, rows: int, activation: int, residual, width: int,
-                  out_dtype: torch.dtype):
-    """Row-wise quantization of ``x2d`` and the grouped product from one library call.  Arguments are taken as
-    they are (the functional layer checks them): ``wq`` [E, N, K] or [N, K] with 16-byte row pitch."""
-    dev = x2d.device
-    k = x2d.shape[1]
-    if wq.dim() == 3:
-        groups, n, ldw, stride = wq.shape[0], wq.shape[1], wq.stride(1), wq.stride(0)
+_get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _call_on(dev: torch.device, fn, *args) -> None:
+    """``fn(*args, stream)`` with ``dev`` current, on its current stream (no context manager in the usual case)."""
+    index = dev.index
+    if index is None or index == _get_device():
+        rc = fn(*args, _stream(dev))
     else:
-        groups, n, ldw, stride = 1, wq.shape[0], wq.stride(0), 0
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream(dev))
+    if rc:
+        check(rc)
+
+
+# The three entry points below are what the functional layer calls once per operator; it has checked the arguments
+# (CUDA tensors of one device with dense rows, contiguous parameters), which are taken as they are.
+def expert_linear(x2d, wq, sw, bias, positions, offsets, rows: int, activation: int, residual, width: int,
+                  out_dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
+    """Row-wise quantization of ``x2d`` and the product with ``wq`` [E, N, K] or [N, K] (16-byte row pitch) from one
+    library call (``lc_expert_linear``)."""
+    x_rows, k = x2d.shape
+    strides = wq.stride()
+    shape = wq.shape
+    if len(shape) == 3:
+        groups, n, ldw, stride = shape[0], shape[1], strides[1], strides[0]
+    else:
+        groups, n, ldw, stride = 1, shape[0], strides[0], 0
     out = torch.empty((rows, width), dtype=out_dtype, device=dev)
-    need = (rows * _pad16(k) + 255) // 256 * 256 + (rows * 4 + 255) // 256 * 256  # lc_expert_linear_workspace_bytes
+    need = (rows * ((k + 15) & -16) + 255 & -256) + (rows * 4 + 255 & -256)  # lc_expert_linear_workspace_bytes
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        check(_expert_linear(x2d.data_ptr(), _DTYPE[x2d.dtype], x2d.shape[0], x2d.stride(0), _ptr(positions),
-                             1 if positions is None else positions.shape[1], _ptr(offsets), groups, rows, wq.data_ptr(),
-                             ldw, stride, n, k, sw.data_ptr(), _ptr(bias), activation, _ptr(residual),
-                             0 if residual is None else residual.stride(0), out.data_ptr(), _DTYPE[out_dtype], width,
-                             ws.data_ptr(), need, None, _stream(dev)))
+    _call_on(dev, _expert_linear, x2d.data_ptr(), _DTYPE[x2d.dtype], x_rows, x2d.stride(0),
+             None if positions is None else positions.data_ptr(), 1 if positions is None else positions.shape[1],
+             None if offsets is None else offsets.data_ptr(), groups, rows, wq.data_ptr(), ldw, stride, n, k,
+             sw.data_ptr(), None if bias is None else bias.data_ptr(), activation,
+             None if residual is None else residual.data_ptr(), 0 if residual is None else residual.stride(0),
+             out.data_ptr(), _DTYPE[out_dtype], width, ws.data_ptr(), need, None)
     return out
+
+
+_ROUTE_ONE_CTA = 128  # tokens up to which lc_route_experts needs no workspace
 
 
 def route_experts(logits, top_k: int, renormalize: bool):
     """``(weights, experts, offsets, positions)`` of the router (``lc_route_experts``)."""
-    dev = _need_cuda(logits)
+    dev = logits.device
     if logits.stride(1) != 1:
         logits = logits.contiguous()
     t, e = logits.shape
@@ -433,24 +454,24 @@ def route_experts(logits, top_k: int, renormalize: bool):
     experts = torch.empty((t, top_k), dtype=torch.int32, device=dev)
     positions = torch.empty((t, top_k), dtype=torch.int32, device=dev)
     offsets = torch.empty(e + 1, dtype=torch.int32, device=dev)
-    need = int(lib.lc_route_experts_workspace_bytes(t, e))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    with _on(dev):
-        check(_route_experts(logits.data_ptr(), _lc_dtype(logits.dtype), t, e, logits.stride(0), top_k,
-                             1 if renormalize else 0, weights.data_ptr(), experts.data_ptr(), offsets.data_ptr(),
-                             positions.data_ptr(), _ptr(ws), need, _stream(dev)))
+    ws, need = None, 0
+    if t > _ROUTE_ONE_CTA:
+        need = int(lib.lc_route_experts_workspace_bytes(t, e))
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _call_on(dev, _route_experts, logits.data_ptr(), _DTYPE[logits.dtype], t, e, logits.stride(0), top_k,
+             1 if renormalize else 0, weights.data_ptr(), experts.data_ptr(), offsets.data_ptr(), positions.data_ptr(),
+             None if ws is None else ws.data_ptr(), need)
     return weights, experts, offsets, positions
 
 
-def combine_experts(y, weights, positions, residual=None):
+def combine_experts(y, weights, positions, residual, dev: torch.device) -> torch.Tensor:
     """``sum_j weights[t, j] * y[positions[t, j]] (+ residual[t])`` (``lc_combine_experts``)."""
-    dev = _need_cuda(y, weights, positions, residual)
     t, top_k = positions.shape
-    out = torch.empty((t, y.shape[1]), dtype=y.dtype, device=dev)
-    with _on(dev):
-        check(_combine_experts(y.data_ptr(), _DTYPE[y.dtype], y.shape[0], y.shape[1], y.stride(0), weights.data_ptr(),
-                               positions.data_ptr(), t, top_k, _ptr(residual),
-                               0 if residual is None else residual.stride(0), out.data_ptr(), y.shape[1], _stream(dev)))
+    rows, cols = y.shape
+    out = torch.empty((t, cols), dtype=y.dtype, device=dev)
+    _call_on(dev, _combine_experts, y.data_ptr(), _DTYPE[y.dtype], rows, cols, y.stride(0), weights.data_ptr(),
+             positions.data_ptr(), t, top_k, None if residual is None else residual.data_ptr(),
+             0 if residual is None else residual.stride(0), out.data_ptr(), cols)
     return out
 
 

@@ -80,14 +80,13 @@ def pack_weight(codes: torch.Tensor) -> torch.Tensor:
     """The int8 codes ``[..., N, K]`` with rows on 16-byte boundaries, which is what the products read:
     ``codes`` itself when they are already, else a view into a padded copy.  Call it once per weight;
     :func:`linear` and :func:`expert_linear` make the copy on every call for a weight that needs it."""
-    if codes.dtype != torch.int8:
+    if codes.dtype is not torch.int8:
         raise TypeError(f"weight codes must be int8, got {codes.dtype}")
-    if codes.dim() < 2:
+    strides = codes.stride()
+    if len(strides) < 2:
         raise ValueError("weight codes must have at least two dimensions [N, K]")
     k = codes.shape[-1]
-    pitched = all(s % 16 == 0 for s, d in zip(codes.stride()[:-1], codes.shape[:-1]) if d > 1)
-    if codes.stride(-1) == 1 and pitched and codes.stride(-2) >= k and codes.stride(-2) % 16 == 0 \
-            and codes.data_ptr() % 16 == 0:
+    if strides[-1] == 1 and strides[-2] >= k and not any(s & 15 for s in strides[:-1]) and codes.data_ptr() & 15 == 0:
         return codes
     store = codes.new_zeros((*codes.shape[:-1], (k + 15) // 16 * 16))
     store[..., :k] = codes
@@ -100,21 +99,32 @@ def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
         raise TypeError(f"{what} must be float32, bfloat16 or float16, got {x.dtype}")
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1])
-    if x.stride(1) != 1 or x.stride(0) < x.shape[1]:
-        x = x.contiguous()
-    return x
+    strides = x.stride()
+    return x if strides[1] == 1 and strides[0] >= x.shape[1] else x.contiguous()
 
 
 def _vector(t: torch.Tensor | None, shape: tuple, name: str, device: torch.device):
     if t is None:
         return None
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
     if t.device != device:
         raise RuntimeError(f"tensors on different devices: {device} and {t.device}")
-    if t.dtype != torch.float32:
+    if t.dtype is not torch.float32:
         t = t.float()
     return t if t.is_contiguous() else t.contiguous()
+
+
+def _residual(t: torch.Tensor | None, shape: tuple, dtype: torch.dtype, device: torch.device):
+    if t is None:
+        return None
+    if t.shape != shape:
+        raise ValueError(f"residual has shape {tuple(t.shape)}, expected {shape}")
+    if t.dtype is not dtype:
+        raise TypeError(f"residual must have the result's type {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise RuntimeError(f"tensors on different devices: {device} and {t.device}")
+    return _rows(t, "residual")
 
 
 def _activation(name, n: int) -> int:
@@ -127,12 +137,20 @@ def _activation(name, n: int) -> int:
     return code
 
 
-def _check_cuda(x: torch.Tensor, weight: torch.Tensor) -> None:
-    if not x.is_cuda and not hasattr(_backend.ops(), "runs_on_cpu"):
+def _check_cuda(x: torch.Tensor, device: torch.device) -> None:
+    if not x.is_cuda:
         raise RuntimeError("the quantized kernels take CUDA tensors only (there is no CPU fallback); "
                            f"got a tensor on {x.device}")
-    if weight.device != x.device:
-        raise RuntimeError(f"tensors on different devices: {x.device} and {weight.device}")
+    if device != x.device:
+        raise RuntimeError(f"tensors on different devices: {x.device} and {device}")
+
+
+def _result_type(x: torch.Tensor, out_dtype) -> torch.dtype:
+    if out_dtype is None:
+        return x.dtype
+    if out_dtype not in _FLOATS:
+        raise TypeError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
+    return out_dtype
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -151,29 +169,22 @@ def linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bi
     n, k = weight.shape
     if x.dim() < 1 or x.shape[-1] != k:
         raise ValueError(f"input of shape {tuple(x.shape)} does not contract with a [{n}, {k}] weight")
-    _check_cuda(x, weight)
+    device = x.device
+    _check_cuda(x, weight.device)
     x2 = _rows(x, "input")
     act = _activation(activation, n)
-    dtype = x.dtype if out_dtype is None else out_dtype
-    if dtype not in _FLOATS:
-        raise TypeError(f"out_dtype must be float32, bfloat16 or float16, got {dtype}")
+    dtype = _result_type(x, out_dtype)
     width = n // 2 if activation == "swiglu" else n
     shape = (*x.shape[:-1], width)
-    if residual is not None:
-        if tuple(residual.shape) != shape:
-            raise ValueError(f"residual has shape {tuple(residual.shape)}, expected {shape}")
-        if residual.dtype != dtype:
-            raise TypeError(f"residual must have the result's type {dtype}, got {residual.dtype}")
-        if residual.device != x.device:
-            raise RuntimeError(f"tensors on different devices: {x.device} and {residual.device}")
-        residual = _rows(residual, "residual")
-    scale = _vector(weight_scale, (n,), "weight_scale", x.device)
-    bias = _vector(bias, (n,), "bias", x.device)
+    residual = _residual(residual, shape, dtype, device)
+    scale = _vector(weight_scale, (n,), "weight_scale", device)
+    bias = _vector(bias, (n,), "bias", device)
     rows = x2.shape[0]
     if rows == 0 or n == 0:
-        return torch.empty(shape, dtype=dtype, device=x.device)
-    y = _backend.ops().expert_linear(x2, pack_weight(weight), scale, bias, None, None, rows, act, residual, width, dtype)
-    return y if x.dim() == 2 else y.view(shape)
+        return torch.empty(shape, dtype=dtype, device=device)
+    y = _backend.ops().expert_linear(x2, pack_weight(weight), scale, bias, None, None, rows, act, residual, width, dtype,
+                                     device)
+    return y if x2 is x else y.view(shape)
 
 
 def route_experts(logits: torch.Tensor, top_k: int, *, renormalize: bool = True) -> ExpertRouting:
@@ -192,7 +203,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, renormalize: bool = True)
     if not 1 <= top_k <= min(count, 32) or count > 1024:
         raise ValueError(f"route_experts: 1 <= top_k <= min(num_experts, 32) and num_experts <= 1024 are required, "
                          f"got top_k = {top_k} of {count}")
-    _check_cuda(logits, logits)
+    _check_cuda(logits, logits.device)
     routing = ExpertRouting.__new__(ExpertRouting)
     routing.weights, routing.experts, routing.offsets, routing.positions = _backend.ops().route_experts(
         logits, top_k, renormalize)
@@ -221,21 +232,19 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Ten
     expected = rows if sorted_rows else routing.tokens
     if x.dim() != 2 or x.shape[0] != expected or x.shape[1] != k:
         raise ValueError(f"input has shape {tuple(x.shape)}, expected ({expected}, {k})")
-    _check_cuda(x, weight)
-    if routing.positions.device != x.device:
-        raise RuntimeError(f"tensors on different devices: {x.device} and {routing.positions.device}")
+    device = x.device
+    _check_cuda(x, weight.device)
+    _check_cuda(x, routing.positions.device)
     x2 = _rows(x, "input")
     act = _activation(activation, n)
-    dtype = x.dtype if out_dtype is None else out_dtype
-    if dtype not in _FLOATS:
-        raise TypeError(f"out_dtype must be float32, bfloat16 or float16, got {dtype}")
+    dtype = _result_type(x, out_dtype)
     width = n // 2 if activation == "swiglu" else n
-    scale = _vector(weight_scale, (e, n), "weight_scale", x.device)
-    bias = _vector(bias, (e, n), "bias", x.device)
+    scale = _vector(weight_scale, (e, n), "weight_scale", device)
+    bias = _vector(bias, (e, n), "bias", device)
     if rows == 0 or n == 0:
-        return torch.empty((rows, width), dtype=dtype, device=x.device)
+        return torch.empty((rows, width), dtype=dtype, device=device)
     return _backend.ops().expert_linear(x2, pack_weight(weight), scale, bias, None if sorted_rows else routing.positions,
-                                        routing.offsets, rows, act, None, width, dtype)
+                                        routing.offsets, rows, act, None, width, dtype, device)
 
 
 def combine_experts(y: torch.Tensor, routing: ExpertRouting, *, residual: torch.Tensor | None = None) -> torch.Tensor:
@@ -244,20 +253,14 @@ def combine_experts(y: torch.Tensor, routing: ExpertRouting, *, residual: torch.
     to the type of ``y``, which ``residual`` [tokens, N] must have too."""
     if y.dim() != 2 or y.shape[0] != routing.rows:
         raise ValueError(f"y has shape {tuple(y.shape)}, expected ({routing.rows}, N)")
-    _check_cuda(y, routing.positions)
+    device = y.device
+    _check_cuda(y, routing.positions.device)
     y = _rows(y, "y")
     shape = (routing.tokens, y.shape[1])
-    if residual is not None:
-        if tuple(residual.shape) != shape:
-            raise ValueError(f"residual has shape {tuple(residual.shape)}, expected {shape}")
-        if residual.dtype != y.dtype:
-            raise TypeError(f"residual must have the type of y, {y.dtype}, got {residual.dtype}")
-        if residual.device != y.device:
-            raise RuntimeError(f"tensors on different devices: {y.device} and {residual.device}")
-        residual = _rows(residual, "residual")
+    residual = _residual(residual, shape, y.dtype, device)
     if shape[0] == 0 or shape[1] == 0:
-        return torch.empty(shape, dtype=y.dtype, device=y.device)
-    return _backend.ops().combine_experts(y, routing.weights, routing.positions, residual)
+        return torch.empty(shape, dtype=y.dtype, device=device)
+    return _backend.ops().combine_experts(y, routing.weights, routing.positions, residual, device)
 
 
 __all__ = ["ACTIVATIONS", "ExpertRouting", "pack_weight", "linear", "route_experts", "expert_linear", "combine_experts"]

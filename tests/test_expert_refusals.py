@@ -126,7 +126,7 @@ def test_c_entry_points_refuse_before_they_launch():
     assert product(groups=2) == invalid and "offsets" in capi.last_error()
     assert product(groups=2, offsets=p, stride=16) == invalid
     assert product(groups=1025, offsets=p) == unsupported
-    assert product(zx=p) == invalid and product(act=6) == invalid and product(variant=3) == invalid
+    assert product(zx=p) == invalid and product(act=6) == invalid and product(variant=7) == invalid
     assert product(act=5, n=24, ldo=24) == invalid and product(dtype=capi.LC_S8) == unsupported
     assert product(ldw=40) == unsupported and product(q=p + 8) == unsupported and product(ldo=8) == invalid
     assert product(k=65552, ldq=65552, ldw=65552) == unsupported and "overflow" in capi.last_error()

@@ -205,7 +205,7 @@ SHAPES = [(1, 1, 1), (1, 16, 64), (3, 130, 100), (16, 256, 512), (17, 128, 4096)
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
-@pytest.mark.parametrize("variant", [1, 2])
+@pytest.mark.parametrize("variant", [1, 2, 3, 4, 5, 6])
 @pytest.mark.parametrize("unsigned", [False, True])
 def test_product_is_exact_in_both_forms(ops, m, n, k, variant, unsigned):
     """With unit scales and fp32 results the product is the integer sum rounded once."""
@@ -404,7 +404,7 @@ def test_expert_linear(F, case, dtype, activation, n, k, sorted_rows):
     assert (y[at:] == 0).all()
 
 
-@pytest.mark.parametrize("variant", [1, 2])
+@pytest.mark.parametrize("variant", [1, 2, 3, 4, 5, 6])
 @pytest.mark.parametrize("case", list(COUNTS))
 def test_grouped_product_forms_agree(ops, F, variant, case):
     counts, top_k, extra = COUNTS[case]
@@ -561,7 +561,7 @@ def test_two_graphs_in_flight(F):
     assert all(torch.equal(a, b) for a, b in zip(outs, want))
 
 
-@pytest.mark.parametrize("variant", [1, 2])
+@pytest.mark.parametrize("variant", [1, 2, 3, 4, 5, 6])
 def test_waits_that_run_out_leave_a_status(ops, variant):
     from lucid_b200._C._loader import LC_QLINEAR_WAIT_TEST, LucidCudaError
 
