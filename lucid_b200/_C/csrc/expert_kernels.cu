@@ -432,6 +432,7 @@ cudaError_t launch_tokens(const TokenParams& p, cudaStream_t st) {
   if (!vec || vectors > 4096) return launch_overlapped(quantize_tokens_any_kernel<T>, grid(1), dim3(256), 0, st, p);
   if (vectors <= 32) return launch_overlapped(quantize_tokens_kernel<T, 32, 1>, grid(8), dim3(256), 0, st, p);
   if (vectors <= 128) return launch_overlapped(quantize_tokens_kernel<T, 32, 4>, grid(8), dim3(256), 0, st, p);
+  if (vectors <= 256) return launch_overlapped(quantize_tokens_kernel<T, 64, 4>, grid(4), dim3(256), 0, st, p);
   if (vectors <= 512) return launch_overlapped(quantize_tokens_kernel<T, 128, 4>, grid(2), dim3(256), 0, st, p);
   if (vectors <= 1024) return launch_overlapped(quantize_tokens_kernel<T, 256, 4>, grid(1), dim3(256), 0, st, p);
   if (vectors <= 2048) return launch_overlapped(quantize_tokens_kernel<T, 512, 4>, grid(1), dim3(512), 0, st, p);

@@ -17,7 +17,7 @@
 // Two forms:
 //  * pair (cta_group::2): 256 weight rows x up to 256 rows of q per tile, each CTA of the pair loading
 //    its own 128 weight rows and half of the q rows; for groups that fill such tiles.
-//  * split (cta_group::1): 128 weight rows x up to 64 rows of q, K cut over the CTAs of a cluster.
+//  * split (cta_group::1): 128 weight rows x up to 16 or 64 rows of q, K cut over the CTAs of a cluster.
 //    Decode batches have few tiles (a [4096, 14336] layer: 32), and a cluster of up to eight gives every
 //    SM a share of the weight's bytes.  The partial sums are int32, so adding them in rank 0's shared
 //    memory in any order gives the same bits.
@@ -45,36 +45,35 @@ constexpr int EPI_WARPS = 8;
 constexpr int EPI_THREADS = EPI_WARPS * 32;
 constexpr int MAX_GROUPS = 1024;
 
-template <int CG>
+// kTokens: rows of q per tile; kStep: granularity of the instruction's N; kBox: rows of q per TMA box of a tile
+// that is not full; kRed: bytes of rank 0's buffer for the other ranks' partial sums, [column][lane]
+template <int FORM>
 struct Cfg;
+constexpr int kSplit16 = 0, kSplit64 = 1, kPair = 2;
 template <>
-struct Cfg<2> {
-  static constexpr int kTile = 256;   // weight rows per tile
-  static constexpr int kTokens = 256; // q rows per tile
-  static constexpr int kStep = 32;    // granularity of the instruction's N
-  static constexpr int kBox = 32;     // q rows per TMA box
-  static constexpr int kStages = 6;
-  static constexpr int kBBytes = (kTokens / 2) * BK;
-  static constexpr int kRedBytes = 0;
+struct Cfg<kSplit16> {
+  static constexpr int kCtas = 1, kTile = 128, kTokens = 16, kStep = 16, kBox = 16, kStages = 11;
+  static constexpr int kBBytes = kTokens * BK, kRed = kTokens * WROWS * 4;
 };
 template <>
-struct Cfg<1> {
-  static constexpr int kTile = 128;
-  static constexpr int kTokens = 64;
-  static constexpr int kStep = 16;
-  static constexpr int kBox = 16;
-  static constexpr int kStages = 7;
-  static constexpr int kBBytes = kTokens * BK;
-  static constexpr int kRedBytes = kTokens * WROWS * 4;  // partial sums of the other ranks, [column][lane]
+struct Cfg<kSplit64> {
+  static constexpr int kCtas = 1, kTile = 128, kTokens = 64, kStep = 16, kBox = 16, kStages = 7;
+  static constexpr int kBBytes = kTokens * BK, kRed = kTokens * WROWS * 4;
 };
-template <int CG>
-__host__ __device__ constexpr int stage_bytes() { return A_BYTES + Cfg<CG>::kBBytes; }
-template <int CG>
+template <>
+struct Cfg<kPair> {
+  static constexpr int kCtas = 2, kTile = 256, kTokens = 256, kStep = 32, kBox = 32, kStages = 6;
+  static constexpr int kBBytes = (kTokens / 2) * BK, kRed = 0;
+};
+template <int FORM>
+__host__ __device__ constexpr int stage_bytes() { return A_BYTES + Cfg<FORM>::kBBytes; }
+template <int FORM>
 __host__ __device__ constexpr int smem_bytes() {
-  return 1024 + Cfg<CG>::kStages * stage_bytes<CG>() + 256 + Cfg<CG>::kRedBytes + 2 * Cfg<CG>::kTokens * 4 +
+  return 1024 + Cfg<FORM>::kStages * stage_bytes<FORM>() + 256 + Cfg<FORM>::kRed + 2 * Cfg<FORM>::kTokens * 4 +
          2 * (MAX_GROUPS + 1) * 4;
 }
-static_assert(smem_bytes<1>() <= 232448 && smem_bytes<2>() <= 232448, "shared memory of a CTA");
+static_assert(smem_bytes<kSplit16>() <= 232448 && smem_bytes<kSplit64>() <= 232448 && smem_bytes<kPair>() <= 232448,
+              "shared memory of a CTA");
 
 enum : int { ST_PRODUCER = 1, ST_MMA = 2, ST_EPILOGUE = 3 };
 
@@ -96,6 +95,7 @@ struct Params {
   int64_t ldo;
   int32_t* status;
   int wait_test;
+  int tokens;               // rows of q per tile, at most the form's kTokens
   int split;                // CTAs of a cluster that share a tile's K (CG == 1)
   int early_weights;        // the weight and offsets were complete before the previous kernel began
   uint32_t idesc;           // instruction descriptor without its N field
@@ -128,8 +128,15 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity,
 __device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-__device__ __forceinline__ void red_add_cluster(uint32_t cluster_addr, uint32_t v) {
-  asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+// adds to a word of another CTA's shared memory and counts four bytes on that CTA's mbarrier once it is there
+__device__ __forceinline__ void red_add_async(uint32_t cluster_addr, uint32_t v, uint32_t cluster_bar) {
+  asm volatile("red.async.relaxed.cluster.shared::cluster.mbarrier::complete_tx::bytes.add.u32 [%0], %1, [%2];" ::"r"(
+                   cluster_addr),
+               "r"(v), "r"(cluster_bar)
+               : "memory");
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
   asm volatile(
@@ -177,16 +184,17 @@ struct Tile {
 
 // Tiles are numbered group by group; within a group, bands of 16 row tiles share the weight tiles.  The walk
 // only moves forward because a CTA's tile numbers grow.
-template <int CG>
+template <int FORM>
 struct TileWalk {
   const int* start;  // [E + 1] first tile of each group
   const int* off;    // [E + 1] first row of each group
-  int tiles_n, e;
-  __device__ __forceinline__ TileWalk(const int* s, const int* o, int tn) : start(s), off(o), tiles_n(tn), e(0) {}
+  int tiles_n, tokens, e;
+  __device__ __forceinline__ TileWalk(const int* s, const int* o, int tn, int tt)
+      : start(s), off(o), tiles_n(tn), tokens(tt), e(0) {}
   __device__ __forceinline__ Tile at(int t) {
     while (t >= start[e + 1]) ++e;
     const int rows = off[e + 1] - off[e];
-    const int tiles_m = (rows + Cfg<CG>::kTokens - 1) / Cfg<CG>::kTokens;
+    const int tiles_m = (rows + tokens - 1) / tokens;
     const int local = t - start[e];
     constexpr int kBand = 16;
     const int band = kBand * tiles_n;
@@ -196,10 +204,10 @@ struct TileWalk {
     const int tm = first + r % gm, tn = r / gm;
     Tile tile;
     tile.e = e;
-    tile.m0 = off[e] + tm * Cfg<CG>::kTokens;
+    tile.m0 = off[e] + tm * tokens;
     const int left = off[e + 1] - tile.m0;
-    tile.rows = left < Cfg<CG>::kTokens ? left : Cfg<CG>::kTokens;
-    tile.n0 = static_cast<int64_t>(tn) * Cfg<CG>::kTile;
+    tile.rows = left < tokens ? left : tokens;
+    tile.n0 = static_cast<int64_t>(tn) * Cfg<FORM>::kTile;
     return tile;
   }
 };
@@ -344,13 +352,14 @@ __device__ __forceinline__ void drain(const Params& p, const Lane& l) {
   }
 }
 
-template <int CG, typename T, int ACT>
+template <int FORM, typename T, int ACT>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_q,
                       const __grid_constant__ CUtensorMap tmap_q_full, const Params p) {
-  using C = Cfg<CG>;
-  constexpr int STAGES = C::kStages, STAGE_BYTES = stage_bytes<CG>();
-  constexpr int TMEM_COLS = 2 * C::kTokens;  // 512 or 128
+  using C = Cfg<FORM>;
+  constexpr int CG = C::kCtas;
+  constexpr int STAGES = C::kStages, STAGE_BYTES = stage_bytes<FORM>();
+  constexpr int TMEM_COLS = 2 * C::kTokens;  // 32, 128 or 512
   static_assert(2 * STAGES * 8 + 6 * 8 <= 256, "barrier area");
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint32_t s_tmem_base;
@@ -361,7 +370,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   const uint32_t red_base = bar_base + 256;
   uint8_t* const after = smem_raw + (red_base - smem_u32(smem_raw));
   int* const s_red = reinterpret_cast<int*>(after);
-  float* const s_sx = reinterpret_cast<float*>(after + C::kRedBytes);  // two accumulator stages
+  float* const s_sx = reinterpret_cast<float*>(after + C::kRed);  // two accumulator stages
   int* const s_off = reinterpret_cast<int*>(s_sx + 2 * C::kTokens);
   int* const s_start = s_off + (MAX_GROUPS + 1);
   auto full_bar = [&](int s) { return bar_base + 8u * s; };
@@ -382,44 +391,36 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   const int kb0 = CG == 2 ? 0 : static_cast<int>(static_cast<int64_t>(num_kb) * rank / p.split);
   const int kb1 = CG == 2 ? num_kb : static_cast<int>(static_cast<int64_t>(num_kb) * (rank + 1) / p.split);
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(full_bar(s), 1);
-      mbar_init(empty_bar(s), 1);
+  // Warp 0 sets up the barriers and the tile table and, in the split form, requests the first weights before the
+  // rest of the CTA is ready (its copies touch no barrier but this CTA's own); warp 1 allocates TMEM meanwhile.
+  uint32_t armed = 0, armed_parity = 0;  // producer: stages with copies in flight, one bit each
+  int ahead = 0;                         // producer: stages whose weights have been requested
+  if (warp == 0) {
+    if (lane < STAGES) {
+      mbar_init(full_bar(lane), 1);
+      mbar_init(empty_bar(lane), 1);
+    } else if (lane < STAGES + 2) {
+      mbar_init(acc_full_bar(lane - STAGES), 1);
+      mbar_init(acc_empty_bar(lane - STAGES), CG * EPI_WARPS);
+    } else if (lane == STAGES + 2) {
+      mbar_init(part_bar, 1);
+      mbar_init(free_bar, EPI_WARPS);
+    } else if (lane == 31) {
+      prefetch_map(&tmap_w);
+      prefetch_map(&tmap_q);
+      prefetch_map(&tmap_q_full);
     }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(acc_full_bar(s), 1);
-      mbar_init(acc_empty_bar(s), CG * EPI_WARPS);
-    }
-    mbar_init(part_bar, p.split > 1 ? (p.split - 1) * EPI_WARPS : 1);
-    mbar_init(free_bar, EPI_WARPS);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == 1) {
-    if constexpr (CG == 2) {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)),
-                   "r"(static_cast<uint32_t>(TMEM_COLS))
-                   : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    } else {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)),
-                   "r"(static_cast<uint32_t>(TMEM_COLS))
-                   : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-  }
-  if (C::kRedBytes > 0 && p.split > 1 && leader)
-    for (int i = threadIdx.x; i < C::kRedBytes / 4; i += NUM_THREADS) s_red[i] = 0;
-
-  if (!p.early_weights) pdl_wait();
-  // first row and first tile of every group (clamped to the rows there are: offsets come from the caller)
-  if (warp == 2) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the copies below count on them at once
+    __syncwarp();
+    if (!p.early_weights) pdl_wait();
+    // first row and first tile of every group (clamped to the rows there are: offsets come from the caller)
     if (!p.offsets) {
       if (lane == 0) {
         s_off[0] = 0;
         s_off[1] = static_cast<int>(p.R);
         s_start[0] = 0;
-        s_start[1] = static_cast<int>((p.R + C::kTokens - 1) / C::kTokens) * tiles_n;
+        s_start[1] = static_cast<int>((p.R + p.tokens - 1) / p.tokens) * tiles_n;
       }
     } else {
       const int R = static_cast<int>(p.R);
@@ -429,7 +430,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         int tiles = 0;
         if (e < p.E) {
           const int a = min(max(p.offsets[e], 0), R), b = min(max(p.offsets[e + 1], a), R);
-          tiles = (b - a + C::kTokens - 1) / C::kTokens * tiles_n;
+          tiles = (b - a + p.tokens - 1) / p.tokens * tiles_n;
           s_off[e] = a;
           if (e == p.E - 1) s_off[p.E] = b;
         }
@@ -444,10 +445,42 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       }
       if (lane == 0) s_start[0] = 0;
     }
+    // arrive before the copies are issued: the release of the arrival waits for them otherwise (measured: 4 us)
+    __syncwarp();
+    cluster_arrive();
+    if (CG == 1 && lane == 0 && unit < s_start[p.E] && !p.wait_test) {
+      TileWalk<FORM> walk(s_start, s_off, tiles_n, p.tokens);
+      const Tile tile = walk.at(unit);
+      const int boxes = (tile.rows + C::kBox - 1) / C::kBox;
+      ahead = min(STAGES, kb1 - kb0);
+      for (int s = 0; s < ahead; ++s) {
+        mbar_expect_tx(full_bar(s), A_BYTES + boxes * C::kBox * BK);
+        tma_load_3d(tiles_base + s * STAGE_BYTES, &tmap_w, (kb0 + s) * BK, static_cast<int>(tile.n0), tile.e, full_bar(s));
+      }
+      armed = (1u << ahead) - 1;
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if constexpr (CG == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)),
+                   "r"(static_cast<uint32_t>(TMEM_COLS))
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)),
+                   "r"(static_cast<uint32_t>(TMEM_COLS))
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+  } else if (CG == 1 && p.split > 1 && leader) {
+    for (int i = threadIdx.x - 64; i < C::kRed / 4; i += EPI_THREADS) s_red[i] = 0;
   }
-  tc_fence_before();
-  __syncthreads();
-  cluster_sync_all();  // the other CTAs' barriers (and rank 0's zeroed buffer) exist before anything reaches them
+  if (warp != 0) {
+    tc_fence_before();
+    __syncwarp();
+    cluster_arrive();
+  }
+  cluster_wait();  // this CTA's set-up and the other CTAs' barriers (and rank 0's zeroed buffer) are complete
   tc_fence_after();
   const uint32_t tmem_base = s_tmem_base;
   const int total = s_start[p.E];
@@ -455,11 +488,11 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   if (warp == 0) {
     // ===================== TMA producer =====================
     if (lane == 0) {
-      uint32_t armed = 0, armed_parity = 0;  // one bit per stage
       int stage = 0;
       uint32_t phase = 0;
-      bool ok = true, waited = !p.early_weights;
-      TileWalk<CG> walk(s_start, s_off, tiles_n);
+      bool ok = true;
+      if (p.early_weights) pdl_wait();  // the codes are the previous kernel's
+      TileWalk<FORM> walk(s_start, s_off, tiles_n, p.tokens);
       for (int t = unit; t < total && ok && !p.wait_test; t += units) {
         const Tile tile = walk.at(t);
         const int cols = (tile.rows + C::kStep - 1) / C::kStep * C::kStep;
@@ -484,7 +517,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         };
         auto load_q = [&](int s, int kb) {
           const uint32_t dst = tiles_base + s * STAGE_BYTES + A_BYTES;
-          if (mine == C::kTokens / CG) {  // a full tile: one box instead of four
+          if (mine == p.tokens / CG) {  // a full tile: one box instead of four
             if constexpr (CG == 2)
               tma_load_2d_pair(dst, &tmap_q_full, kb * BK, m0, map_to_cta(full_bar(s), 0));
             else
@@ -499,15 +532,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
           }
         };
         int kb = kb0;
-        if (!waited) {
-          // the ring is empty: fill it with weights while the kernel before this one still writes the codes
-          const int ahead = min(STAGES, kb1 - kb0);
-          for (int s = 0; s < ahead; ++s) {
-            arm(s, 0);
-            load_w(s, kb0 + s);
-          }
-          pdl_wait();
-          waited = true;
+        if (CG == 1 && t == unit && ahead) {  // the first stages have their weights under way
           for (int s = 0; s < ahead; ++s) load_q(s, kb0 + s);
           kb = kb0 + ahead;
           stage = ahead % STAGES;
@@ -538,7 +563,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       int stage = 0, it = 0;
       uint32_t phase = 0;
       bool ok = true;
-      TileWalk<CG> walk(s_start, s_off, tiles_n);
+      TileWalk<FORM> walk(s_start, s_off, tiles_n, p.tokens);
       for (int t = unit; t < total && ok; t += units, ++it) {
         const Tile tile = walk.at(t);
         const uint32_t cols = (tile.rows + C::kStep - 1) / C::kStep * C::kStep;
@@ -592,7 +617,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     const int et = threadIdx.x - 64;
     if (p.early_weights) pdl_wait();
     const int zx = p.zx ? __float2int_rn(__ldg(p.zx)) : 0;
-    TileWalk<CG> walk(s_start, s_off, tiles_n);
+    TileWalk<FORM> walk(s_start, s_off, tiles_n, p.tokens);
     int it = 0;
     for (int t = unit; t < total; t += units, ++it) {
       const Tile tile = walk.at(t);
@@ -605,6 +630,8 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       const float sw = in ? __ldg(p.sw + at) : 0.0f;
       const float bias = (in && p.bias) ? __ldg(p.bias + at) : 0.0f;
       const int corr = (in && p.wsum) ? zx * __ldg(p.wsum + at) : 0;
+      if (CG == 1 && p.split > 1 && leader && et == 0)
+        mbar_expect_tx(part_bar, static_cast<uint32_t>((p.split - 1) * tile.rows * WROWS * 4));
       bool arrived = mbar_wait(acc_full_bar(as), (it >> 1) & 1, budget);
       if (CG == 1 && p.split > 1)
         arrived = arrived && (leader ? mbar_wait_cluster(part_bar, it & 1, budget)
@@ -612,6 +639,8 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       // also publishes the staged scales; those of the tile before last are no longer read
       if (!epilogue_all(arrived)) {
         report(p.status, ST_EPILOGUE);
+        // sums another rank may still be sending land in this CTA's memory: give them the same time again
+        if (CG == 1 && p.split > 1 && leader) mbar_wait_cluster(part_bar, it & 1, budget);
         break;
       }
       tc_fence_after();
@@ -629,6 +658,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       l.red = CG == 1 && p.split > 1 ? s_red : nullptr;
       if (CG == 1 && !leader) {
         const uint32_t dst = map_to_cta(red_base, 0) + static_cast<uint32_t>(l.slot) * 4;
+        const uint32_t bar = map_to_cta(part_bar, 0);
 #pragma unroll 1
         for (int c = l.first; c < l.rows; c += 2 * CH) {
           uint32_t r[CH];
@@ -636,20 +666,16 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
           tc_wait_ld();
 #pragma unroll
           for (int j = 0; j < CH; ++j)
-            if (c + j < l.rows) red_add_cluster(dst + static_cast<uint32_t>((c + j) * WROWS * 4), r[j]);
+            if (c + j < l.rows) red_add_async(dst + static_cast<uint32_t>((c + j) * WROWS * 4), r[j], bar);
         }
       } else {
         drain<T, ACT>(p, l);
       }
       tc_fence_before();
-      if (CG == 1 && p.split > 1) {
+      if (CG == 1 && p.split > 1 && leader && t + units < total) {  // the cleared buffer may be added to again
         asm volatile("fence.acq_rel.cluster;" ::: "memory");
         __syncwarp();
-        if (!leader) {
-          if (lane == 0) mbar_arrive_release_cluster(map_to_cta(part_bar, 0));
-        } else if (lane > 0 && lane < p.split) {
-          mbar_arrive_release_cluster(map_to_cta(free_bar, lane));
-        }
+        if (lane > 0 && lane < p.split) mbar_arrive_release_cluster(map_to_cta(free_bar, lane));
       }
       __syncwarp();
       if (lane == 0) {
@@ -687,22 +713,34 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
 // ---- host side -------------------------------------------------------------------------------
 using Kernel = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, Params);
 
-template <int CG, typename T>
+template <int FORM, typename T>
 static Kernel kernel_for(int act) {
   switch (act) {
-    case LC_ACT_RELU: return grouped_linear_kernel<CG, T, LC_ACT_RELU>;
-    case LC_ACT_GELU: return grouped_linear_kernel<CG, T, LC_ACT_GELU>;
-    case LC_ACT_GELU_TANH: return grouped_linear_kernel<CG, T, LC_ACT_GELU_TANH>;
-    case LC_ACT_SILU: return grouped_linear_kernel<CG, T, LC_ACT_SILU>;
-    case LC_ACT_SWIGLU: return grouped_linear_kernel<CG, T, LC_ACT_SWIGLU>;
-    default: return grouped_linear_kernel<CG, T, LC_ACT_NONE>;
+    case LC_ACT_RELU: return grouped_linear_kernel<FORM, T, LC_ACT_RELU>;
+    case LC_ACT_GELU: return grouped_linear_kernel<FORM, T, LC_ACT_GELU>;
+    case LC_ACT_GELU_TANH: return grouped_linear_kernel<FORM, T, LC_ACT_GELU_TANH>;
+    case LC_ACT_SILU: return grouped_linear_kernel<FORM, T, LC_ACT_SILU>;
+    case LC_ACT_SWIGLU: return grouped_linear_kernel<FORM, T, LC_ACT_SWIGLU>;
+    default: return grouped_linear_kernel<FORM, T, LC_ACT_NONE>;
   }
 }
-template <int CG>
+template <int FORM>
 static Kernel kernel_for(int dtype, int act) {
-  return dtype == LC_F32    ? kernel_for<CG, float>(act)
-         : dtype == LC_BF16 ? kernel_for<CG, __nv_bfloat16>(act)
-                            : kernel_for<CG, __half>(act);
+  return dtype == LC_F32    ? kernel_for<FORM, float>(act)
+         : dtype == LC_BF16 ? kernel_for<FORM, __nv_bfloat16>(act)
+                            : kernel_for<FORM, __half>(act);
+}
+
+static Kernel kernel_for(int form, int dtype, int act) {
+  return form == kSplit16   ? kernel_for<kSplit16>(dtype, act)
+         : form == kSplit64 ? kernel_for<kSplit64>(dtype, act)
+                            : kernel_for<kPair>(dtype, act);
+}
+static int smem_of(int form) {
+  return form == kSplit16 ? smem_bytes<kSplit16>() : form == kSplit64 ? smem_bytes<kSplit64>() : smem_bytes<kPair>();
+}
+static int tokens_of(int form) {
+  return form == kSplit16 ? Cfg<kSplit16>::kTokens : form == kSplit64 ? Cfg<kSplit64>::kTokens : Cfg<kPair>::kTokens;
 }
 
 static void launch_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attrs, unsigned grid, int smem, int cluster,
@@ -738,19 +776,18 @@ static int32_t device_info(const DeviceInfo** out) {
     DeviceInfo& info = infos[dev];
     info.err = cudaSuccess;
     for (int dtype : {LC_F32, LC_BF16, LC_F16})
-      for (int act = LC_ACT_NONE; act <= LC_ACT_SWIGLU && info.err == cudaSuccess; ++act) {
-        info.err = cudaFuncSetAttribute(kernel_for<1>(dtype, act), cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<1>());
-        if (info.err == cudaSuccess)
-          info.err = cudaFuncSetAttribute(kernel_for<2>(dtype, act), cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<2>());
-      }
+      for (int act = LC_ACT_NONE; act <= LC_ACT_SWIGLU; ++act)
+        for (int form : {kSplit16, kSplit64, kPair})
+          if (info.err == cudaSuccess)
+            info.err = cudaFuncSetAttribute(kernel_for(form, dtype, act), cudaFuncAttributeMaxDynamicSharedMemorySize, smem_of(form));
     const int sms = sm_count();
     for (int i = 0; i < 4 && info.err == cudaSuccess; ++i) {
       cudaLaunchConfig_t cfg;
       cudaLaunchAttribute attrs[2];
-      launch_config(&cfg, attrs, static_cast<unsigned>(sms / (1 << i) << i), smem_bytes<1>(), 1 << i, nullptr);
+      launch_config(&cfg, attrs, static_cast<unsigned>(sms / (1 << i) << i), smem_of(kSplit64), 1 << i, nullptr);
       cfg.numAttrs = 1;
       int n = 0;
-      if (cudaOccupancyMaxActiveClusters(&n, kernel_for<1>(LC_F32, LC_ACT_NONE), &cfg) != cudaSuccess) {
+      if (cudaOccupancyMaxActiveClusters(&n, kernel_for(kSplit64, LC_F32, LC_ACT_NONE), &cfg) != cudaSuccess) {
         cudaGetLastError();
         n = i == 0 ? sms : 0;
       }
@@ -763,35 +800,74 @@ static int32_t device_info(const DeviceInfo** out) {
   return LC_OK;
 }
 
-// Groups whose mean row count exceeds this take the pair form.
-constexpr int64_t kPairRows = 64;
+// Row tiles there can be at most: one partly filled one per group that has rows, the rest full.
+static int64_t row_tiles(const Params& p, int tokens) {
+  const int64_t groups = p.offsets ? (p.E < p.R ? p.E : p.R) : 1;
+  return (p.R - groups) / tokens + groups;
+}
+
+// Form by the rows a group has on average (all that is known on the host).  Above 64 rows the pair's 256 x 256 tiles
+// win once they occupy half of the machine; with fewer of them the narrow tiles spread further ([4096, 4096] weight:
+// 128 rows 18.6 against 20.4 us, 256 rows 21.3 / 22.5, 512 rows 32.8 / 23.3, launch and timing overhead of 7 us
+// included).  Up to 16 rows the smaller code tiles leave room for four more stages of weights in flight.
+static int choose_form(const Params& p, int64_t sms) {
+  if (p.R > 64 * static_cast<int64_t>(p.E)) {
+    const int64_t tiles = row_tiles(p, Cfg<kPair>::kTokens) * ((p.N + 255) / 256);
+    return p.R > 256 * static_cast<int64_t>(p.E) || tiles >= sms / 4 ? kPair : kSplit64;
+  }
+  const int64_t rows = p.offsets ? 2 * p.R : p.R;  // groups differ in size
+  return rows <= 16 * static_cast<int64_t>(p.E) ? kSplit16 : kSplit64;
+}
+
+// Rows of q per tile of the pair form: 256, or fewer where that fills the last wave of tiles better.  Clocks of a tile:
+// a K block takes 2 per row of q on the tensor cores and at least 320 to bring in, the epilogue about 25 per row,
+// beside the next tile's main loop.
+static int pair_tokens(const Params& p, int64_t tiles_n, int num_kb, int64_t units) {
+  int best = 256;
+  int64_t least = 0;
+  for (int tokens : {256, 192, 128}) {
+    const int64_t waves = (row_tiles(p, tokens) * tiles_n + units - 1) / units;
+    const int64_t loop = static_cast<int64_t>(num_kb) * (2 * tokens > 320 ? 2 * tokens : 320), drain = 25 * tokens;
+    const int64_t cost = waves * (loop > drain ? loop : drain) + (loop < drain ? loop : drain);
+    if (tokens == 256 || cost < least - least / 32) {
+      least = cost;
+      best = tokens;
+    }
+  }
+  return best;
+}
 
 static int32_t launch(const void* q, int64_t ldq, const int8_t* w, int64_t ldw, int64_t group_stride, int q_unsigned,
                       Params& p, int variant, cudaStream_t st) {
   const DeviceInfo* info = nullptr;
   if (int32_t rc = device_info(&info)) return rc;
   const int64_t sms = sm_count();
-  const bool pair = variant == 2 || (variant == 0 && p.R > kPairRows * p.E);
+  int form = choose_form(p, sms);
+  if (variant == 2) form = kPair;
+  if (variant != 0 && variant != 2 && form == kPair) form = kSplit64;
+  const bool pair = form == kPair;
   const int forced = variant > 2 ? 1 << (variant - 3) : 0;
+  const int tile_n = pair ? 256 : 128;
+  const int64_t tiles_n = (p.N + tile_n - 1) / tile_n;
+  const int num_kb = static_cast<int>((p.K + BK - 1) / BK);
+  int tokens = tokens_of(form);
+  if (pair) tokens = pair_tokens(p, tiles_n, num_kb, sms / 2);
+  p.tokens = tokens;
   CUtensorMap map_w, map_q, map_q_full;
   if (int32_t rc = encode_tensor_map_3d(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, p.K, p.N, p.E, ldw, group_stride, BK,
                                         WROWS, CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
   if (int32_t rc = encode_tensor_map_2d(&map_q, CU_TENSOR_MAP_DATA_TYPE_UINT8, q, p.K, p.R, ldq, BK,
-                                        pair ? Cfg<2>::kBox : Cfg<1>::kBox, CU_TENSOR_MAP_SWIZZLE_128B))
+                                        pair ? Cfg<kPair>::kBox : Cfg<kSplit64>::kBox, CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
   if (int32_t rc = encode_tensor_map_2d(&map_q_full, CU_TENSOR_MAP_DATA_TYPE_UINT8, q, p.K, p.R, ldq, BK,
-                                        pair ? Cfg<2>::kTokens / 2 : Cfg<1>::kTokens, CU_TENSOR_MAP_SWIZZLE_128B))
+                                        pair ? tokens / 2 : tokens, CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
   // kind::i8: D s32 (2) in bits [4,6); A (weight, s8 = 1) in [7,10), B (codes, s8 = 1 or u8 = 0) in [10,13); both
   // K-major; N >> 3 in [17,23) is filled in per tile; M >> 4 in [24,29)
   p.idesc = (2u << 4) | (1u << 7) | ((q_unsigned ? 0u : 1u) << 10) |
             (static_cast<uint32_t>((pair ? 256 : 128) >> 4) << 24);
-  const int64_t tile_n = pair ? 256 : 128, tile_m = pair ? 256 : 64;
-  const int64_t tiles_n = (p.N + tile_n - 1) / tile_n;
-  // upper bound of the tiles there can be: one partly filled row tile per group that has rows
-  const int64_t groups = p.offsets ? (p.E < p.R ? p.E : p.R) : 1;
-  const int64_t tiles = tiles_n * ((p.R - groups) / tile_m + groups);
+  const int64_t tiles = row_tiles(p, tokens) * tiles_n;
   if (tiles > 0x7fffffffLL) return fail(LC_ERR_UNSUPPORTED, "grouped_linear: too many tiles");
   int cluster = 2;
   int64_t units = sms / 2;
@@ -799,7 +875,6 @@ static int32_t launch(const void* q, int64_t ldq, const int8_t* w, int64_t ldw, 
   if (!pair) {
     // K split: the waves of tiles over the clusters that fit, times each CTA's share of K; two K blocks of
     // hand-over are charged per split tile
-    const int num_kb = static_cast<int>((p.K + BK - 1) / BK);
     double best = 0.0;
     cluster = 1;
     units = sms;
@@ -819,9 +894,8 @@ static int32_t launch(const void* q, int64_t ldq, const int8_t* w, int64_t ldw, 
   if (units > tiles) units = tiles;
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attrs[2];
-  launch_config(&cfg, attrs, static_cast<unsigned>(units * cluster), pair ? smem_bytes<2>() : smem_bytes<1>(), cluster, st);
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, pair ? kernel_for<2>(p.out_dtype, p.act) : kernel_for<1>(p.out_dtype, p.act),
-                                             map_w, map_q, map_q_full, p);
+  launch_config(&cfg, attrs, static_cast<unsigned>(units * cluster), smem_of(form), cluster, st);
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel_for(form, p.out_dtype, p.act), map_w, map_q, map_q_full, p);
   if (err != cudaSuccess) return fail(LC_ERR_CUDA, "grouped_linear: %s", cudaGetErrorString(err));
   return check_launch("grouped_linear");
 }
