@@ -27,6 +27,7 @@
 // leaves its loop, the CTA waits (bounded) for its own copies in flight, frees its TMEM and returns.
 #include <cuda.h>
 
+#include <cmath>
 #include <mutex>
 
 #include "tcgen05.cuh"
@@ -52,7 +53,7 @@ struct Cfg;
 constexpr int kSplit16 = 0, kSplit64 = 1, kPair = 2;
 template <>
 struct Cfg<kSplit16> {
-  static constexpr int kCtas = 1, kTile = 128, kTokens = 16, kStep = 16, kBox = 16, kStages = 11;
+  static constexpr int kCtas = 1, kTile = 128, kTokens = 16, kStep = 16, kBox = 16, kStages = 9;
   static constexpr int kBBytes = kTokens * BK, kRed = kTokens * WROWS * 4;
 };
 template <>
@@ -96,6 +97,7 @@ struct Params {
   int32_t* status;
   int wait_test;
   int tokens;               // rows of q per tile, at most the form's kTokens
+  int tile_rows;            // weight rows per tile: the form's kTile, or fewer (a multiple of 8) in the split form
   int split;                // CTAs of a cluster that share a tile's K (CG == 1)
   int early_weights;        // the weight and offsets were complete before the previous kernel began
   uint32_t idesc;           // instruction descriptor without its N field
@@ -184,13 +186,12 @@ struct Tile {
 
 // Tiles are numbered group by group; within a group, bands of 16 row tiles share the weight tiles.  The walk
 // only moves forward because a CTA's tile numbers grow.
-template <int FORM>
 struct TileWalk {
   const int* start;  // [E + 1] first tile of each group
   const int* off;    // [E + 1] first row of each group
-  int tiles_n, tokens, e;
-  __device__ __forceinline__ TileWalk(const int* s, const int* o, int tn, int tt)
-      : start(s), off(o), tiles_n(tn), tokens(tt), e(0) {}
+  int tiles_n, tokens, tile_rows, e;
+  __device__ __forceinline__ TileWalk(const int* s, const int* o, int tn, const Params& p)
+      : start(s), off(o), tiles_n(tn), tokens(p.tokens), tile_rows(p.tile_rows), e(0) {}
   __device__ __forceinline__ Tile at(int t) {
     while (t >= start[e + 1]) ++e;
     const int rows = off[e + 1] - off[e];
@@ -207,7 +208,7 @@ struct TileWalk {
     tile.m0 = off[e] + tm * tokens;
     const int left = off[e + 1] - tile.m0;
     tile.rows = left < tokens ? left : tokens;
-    tile.n0 = static_cast<int64_t>(tn) * Cfg<FORM>::kTile;
+    tile.n0 = static_cast<int64_t>(tn) * tile_rows;
     return tile;
   }
 };
@@ -276,6 +277,7 @@ struct Lane {
   int64_t m0;       // first row of q
   int rows;
   int64_t n;        // this lane's weight row inside the group
+  bool in;          // there is such a row in this tile
   float sw, bias;
   int corr;         // zx * wsum
   const float* sx;  // scales of the tile's rows
@@ -291,16 +293,13 @@ struct Lane {
 constexpr int CH = 16;
 template <typename T, int ACT>
 __device__ __forceinline__ void drain(const Params& p, const Lane& l) {
-  const bool in = l.n < p.N;
   const int up = (static_cast<int>(l.n) >> 3) & 1;  // SwiGLU: this lane's weight row is an up row
   const int64_t col = ACT == LC_ACT_SWIGLU ? (((l.n >> 4) << 3) | (l.n & 7)) : l.n;
   const int64_t row0 = l.m0 + (ACT == LC_ACT_SWIGLU ? up : 0);
   const T* const res = static_cast<const T*>(p.residual);
 #pragma unroll 1
   for (int c = l.first; c < l.rows; c += 2 * CH) {
-    uint32_t r[CH];
-    tc_ld(l.t_row + static_cast<uint32_t>(c), r);
-    const int left = in ? l.rows - c : 0;
+    const int left = l.in ? l.rows - c : 0;
     constexpr int kStep = ACT == LC_ACT_SWIGLU ? 2 : 1;  // a lane finishes every row, or every second one
     T rv[CH / kStep];
     if (res) {
@@ -311,6 +310,8 @@ __device__ __forceinline__ void drain(const Params& p, const Lane& l) {
         src += kStep * p.ldr;
       }
     }
+    uint32_t r[CH];
+    tc_ld(l.t_row + static_cast<uint32_t>(c), r);
     tc_wait_ld();
     if (l.red) {
       int* mine = l.red + c * WROWS + l.slot;
@@ -386,7 +387,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   const bool leader = rank == 0;
   const int cluster = CG == 2 ? 2 : p.split;
   const int unit = static_cast<int>(blockIdx.x) / cluster, units = static_cast<int>(gridDim.x) / cluster;
-  const int tiles_n = static_cast<int>((p.N + C::kTile - 1) / C::kTile);
+  const int tiles_n = static_cast<int>((p.N + p.tile_rows - 1) / p.tile_rows);
   const int num_kb = static_cast<int>((p.K + BK - 1) / BK);
   const int kb0 = CG == 2 ? 0 : static_cast<int>(static_cast<int64_t>(num_kb) * rank / p.split);
   const int kb1 = CG == 2 ? num_kb : static_cast<int>(static_cast<int64_t>(num_kb) * (rank + 1) / p.split);
@@ -448,15 +449,18 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     // arrive before the copies are issued: the release of the arrival waits for them otherwise (measured: 4 us)
     __syncwarp();
     cluster_arrive();
-    if (CG == 1 && lane == 0 && unit < s_start[p.E] && !p.wait_test) {
-      TileWalk<FORM> walk(s_start, s_off, tiles_n, p.tokens);
+    if (CG == 1 && unit < s_start[p.E] && !p.wait_test) {
+      TileWalk walk(s_start, s_off, tiles_n, p);
       const Tile tile = walk.at(unit);
-      const int boxes = (tile.rows + C::kBox - 1) / C::kBox;
+      const int n0 = static_cast<int>(tile.n0), boxes = (tile.rows + C::kBox - 1) / C::kBox;
+      const uint32_t bytes = static_cast<uint32_t>((p.tile_rows + boxes * C::kBox) * BK);
       ahead = min(STAGES, kb1 - kb0);
-      for (int s = 0; s < ahead; ++s) {
-        mbar_expect_tx(full_bar(s), A_BYTES + boxes * C::kBox * BK);
-        tma_load_3d(tiles_base + s * STAGE_BYTES, &tmap_w, (kb0 + s) * BK, static_cast<int>(tile.n0), tile.e, full_bar(s));
-      }
+      if (elect_one())
+        for (int s = 0; s < ahead; ++s) {
+          mbar_expect_tx(full_bar(s), bytes);
+          tma_load_3d(tiles_base + s * STAGE_BYTES, &tmap_w, (kb0 + s) * BK, n0, tile.e, full_bar(s));
+        }
+      __syncwarp();
       armed = (1u << ahead) - 1;
     }
     __syncwarp();
@@ -487,127 +491,133 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
 
   if (warp == 0) {
     // ===================== TMA producer =====================
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      if (p.early_weights) pdl_wait();  // the codes are the previous kernel's
-      TileWalk<FORM> walk(s_start, s_off, tiles_n, p.tokens);
-      for (int t = unit; t < total && ok && !p.wait_test; t += units) {
-        const Tile tile = walk.at(t);
-        const int cols = (tile.rows + C::kStep - 1) / C::kStep * C::kStep;
-        const int mine = cols / CG;  // q rows this CTA loads
-        const int boxes = (mine + C::kBox - 1) / C::kBox;
-        const uint32_t bytes = CG * (A_BYTES + boxes * C::kBox * BK);
-        const int n0 = static_cast<int>(tile.n0) + (CG == 2 ? static_cast<int>(rank) * WROWS : 0);
-        const int m0 = tile.m0 + (CG == 2 ? static_cast<int>(rank) * mine : 0);
-        auto arm = [&](int s, uint32_t parity) {
-          if (CG == 1 || leader) {
-            mbar_expect_tx(full_bar(s), bytes);
-            armed |= 1u << s;
-            armed_parity = (armed_parity & ~(1u << s)) | (parity << s);
-          }
-        };
-        auto load_w = [&](int s, int kb) {
-          const uint32_t dst = tiles_base + s * STAGE_BYTES;
+    // The whole warp walks the loop and one elected lane issues: in code that only lane 0 reaches, every operand of
+    // a copy or an MMA is moved to a uniform register first, 70 clocks an instruction.
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    if (p.early_weights) pdl_wait();  // the codes are the previous kernel's
+    TileWalk walk(s_start, s_off, tiles_n, p);
+    for (int t = unit; t < total && ok && !p.wait_test; t += units) {
+      const Tile tile = walk.at(t);
+      const int cols = (tile.rows + C::kStep - 1) / C::kStep * C::kStep;
+      const int mine = cols / CG;  // q rows this CTA loads
+      const bool full = mine == p.tokens / CG;  // one box; else as many of kBox rows as it takes
+      const int boxes = (mine + C::kBox - 1) / C::kBox;
+      const uint32_t bytes = static_cast<uint32_t>((p.tile_rows + CG * (full ? mine : boxes * C::kBox)) * BK);
+      const int n0 = static_cast<int>(tile.n0) + (CG == 2 ? static_cast<int>(rank) * WROWS : 0);
+      const int m0 = tile.m0 + (CG == 2 ? static_cast<int>(rank) * mine : 0);
+      const int e = tile.e;
+      auto load_q = [&](int s, int kb) {
+        const uint32_t dst = tiles_base + s * STAGE_BYTES + A_BYTES;
+        if (full) {
           if constexpr (CG == 2)
-            tma_load_3d_pair(dst, &tmap_w, kb * BK, n0, tile.e, map_to_cta(full_bar(s), 0));
+            tma_load_2d_pair(dst, &tmap_q_full, kb * BK, m0, map_to_cta(full_bar(s), 0));
           else
-            tma_load_3d(dst, &tmap_w, kb * BK, n0, tile.e, full_bar(s));
-        };
-        auto load_q = [&](int s, int kb) {
-          const uint32_t dst = tiles_base + s * STAGE_BYTES + A_BYTES;
-          if (mine == p.tokens / CG) {  // a full tile: one box instead of four
-            if constexpr (CG == 2)
-              tma_load_2d_pair(dst, &tmap_q_full, kb * BK, m0, map_to_cta(full_bar(s), 0));
-            else
-              tma_load_2d(dst, &tmap_q_full, kb * BK, m0, full_bar(s));
-            return;
-          }
-          for (int b = 0; b < boxes; ++b) {
-            if constexpr (CG == 2)
-              tma_load_2d_pair(dst + b * C::kBox * BK, &tmap_q, kb * BK, m0 + b * C::kBox, map_to_cta(full_bar(s), 0));
-            else
-              tma_load_2d(dst + b * C::kBox * BK, &tmap_q, kb * BK, m0 + b * C::kBox, full_bar(s));
-          }
-        };
-        int kb = kb0;
-        if (CG == 1 && t == unit && ahead) {  // the first stages have their weights under way
-          for (int s = 0; s < ahead; ++s) load_q(s, kb0 + s);
-          kb = kb0 + ahead;
-          stage = ahead % STAGES;
-          phase = ahead == STAGES ? 1u : 0u;
+            tma_load_2d(dst, &tmap_q_full, kb * BK, m0, full_bar(s));
+          return;
         }
-        for (; kb < kb1; ++kb) {
-          if (!mbar_wait(empty_bar(stage), phase ^ 1u, budget)) {
-            report(p.status, ST_PRODUCER);
-            ok = false;
-            break;
-          }
-          arm(stage, phase);
-          load_w(stage, kb);
+        for (int b = 0; b < boxes; ++b) {
+          if constexpr (CG == 2)
+            tma_load_2d_pair(dst + b * C::kBox * BK, &tmap_q, kb * BK, m0 + b * C::kBox, map_to_cta(full_bar(s), 0));
+          else
+            tma_load_2d(dst + b * C::kBox * BK, &tmap_q, kb * BK, m0 + b * C::kBox, full_bar(s));
+        }
+      };
+      int kb = kb0;
+      if (CG == 1 && t == unit && ahead) {  // the first stages have their weights under way
+        if (elect_one())
+          for (int s = 0; s < ahead; ++s) load_q(s, kb0 + s);
+        __syncwarp();
+        kb = kb0 + ahead;
+        stage = ahead % STAGES;
+        phase = ahead == STAGES ? 1u : 0u;
+      }
+      for (; kb < kb1; ++kb) {
+        if (!__all_sync(0xffffffffu, mbar_wait(empty_bar(stage), phase ^ 1u, budget))) {
+          if (lane == 0) report(p.status, ST_PRODUCER);
+          ok = false;
+          break;
+        }
+        if (elect_one()) {
+          const uint32_t dst = tiles_base + stage * STAGE_BYTES;
+          if (CG == 1 || leader) mbar_expect_tx(full_bar(stage), bytes);
+          if constexpr (CG == 2)
+            tma_load_3d_pair(dst, &tmap_w, kb * BK, n0, e, map_to_cta(full_bar(stage), 0));
+          else
+            tma_load_3d(dst, &tmap_w, kb * BK, n0, e, full_bar(stage));
           load_q(stage, kb);
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
+        }
+        __syncwarp();
+        if (CG == 1 || leader) {
+          armed |= 1u << stage;
+          armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
+        }
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
         }
       }
-      // do not leave while a bulk copy may still be landing (a pair's leader counts the bytes of both CTAs)
-      for (int s = 0; s < STAGES; ++s)
-        if (armed >> s & 1) mbar_wait(full_bar(s), armed_parity >> s & 1);
     }
+    // do not leave while a bulk copy may still be landing (a pair's leader counts the bytes of both CTAs)
+    for (int s = 0; s < STAGES; ++s)
+      if (armed >> s & 1) mbar_wait(full_bar(s), armed_parity >> s & 1);
+    __syncwarp();
   } else if (warp == 1) {
     // ===================== MMA issuer (a pair's leader only) =====================
-    if ((CG == 1 || leader) && lane == 0) {
+    if (CG == 1 || leader) {
       int stage = 0, it = 0;
       uint32_t phase = 0;
       bool ok = true;
-      TileWalk<FORM> walk(s_start, s_off, tiles_n, p.tokens);
+      TileWalk walk(s_start, s_off, tiles_n, p);
       for (int t = unit; t < total && ok; t += units, ++it) {
         const Tile tile = walk.at(t);
         const uint32_t cols = (tile.rows + C::kStep - 1) / C::kStep * C::kStep;
         const uint32_t idesc = p.idesc | ((cols >> 3) << 17);
         const int as = it & 1;
-        if (!mbar_wait(acc_empty_bar(as), ((it >> 1) & 1) ^ 1u, budget)) {
-          report(p.status, ST_MMA);
+        if (!__all_sync(0xffffffffu, mbar_wait(acc_empty_bar(as), ((it >> 1) & 1) ^ 1u, budget))) {
+          if (lane == 0) report(p.status, ST_MMA);
           break;
         }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(as * C::kTokens);
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait(full_bar(stage), phase, budget)) {
-            report(p.status, ST_MMA);
+          if (!__all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase, budget))) {
+            if (lane == 0) report(p.status, ST_MMA);
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t src = tiles_base + stage * STAGE_BYTES;
-          const uint64_t w_desc = make_smem_desc(src), q_desc = make_smem_desc(src + A_BYTES);
+          if (elect_one()) {
+            const uint32_t src = tiles_base + stage * STAGE_BYTES;
+            const uint64_t w_desc = make_smem_desc(src), q_desc = make_smem_desc(src + A_BYTES);
 #pragma unroll
-          for (int j = 0; j < BK / UMMA_K; ++j) {
-            const uint64_t koff = static_cast<uint64_t>((j * UMMA_K) >> 4);
-            const uint32_t accumulate = (kb != kb0 || j != 0) ? 1u : 0u;
+            for (int j = 0; j < BK / UMMA_K; ++j) {
+              const uint64_t koff = static_cast<uint64_t>((j * UMMA_K) >> 4);
+              const uint32_t accumulate = (kb != kb0 || j != 0) ? 1u : 0u;
+              if constexpr (CG == 2)
+                tc_mma_i8_pair(d_tmem, w_desc + koff, q_desc + koff, idesc, accumulate);
+              else
+                tc_mma_i8(d_tmem, w_desc + koff, q_desc + koff, idesc, accumulate);
+            }
             if constexpr (CG == 2)
-              tc_mma_i8_pair(d_tmem, w_desc + koff, q_desc + koff, idesc, accumulate);
+              tc_commit_pair(empty_bar(stage));
             else
-              tc_mma_i8(d_tmem, w_desc + koff, q_desc + koff, idesc, accumulate);
+              tc_commit(empty_bar(stage));
           }
-          if constexpr (CG == 2)
-            tc_commit_pair(empty_bar(stage));
-          else
-            tc_commit(empty_bar(stage));
+          __syncwarp();
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1u;
           }
         }
-        if (ok) {
+        if (ok && elect_one()) {
           if constexpr (CG == 2)
             tc_commit_pair(acc_full_bar(as));
           else
             tc_commit(acc_full_bar(as));
         }
+        __syncwarp();
       }
     }
   } else {
@@ -617,7 +627,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     const int et = threadIdx.x - 64;
     if (p.early_weights) pdl_wait();
     const int zx = p.zx ? __float2int_rn(__ldg(p.zx)) : 0;
-    TileWalk<FORM> walk(s_start, s_off, tiles_n, p.tokens);
+    TileWalk walk(s_start, s_off, tiles_n, p);
     int it = 0;
     for (int t = unit; t < total; t += units, ++it) {
       const Tile tile = walk.at(t);
@@ -626,7 +636,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       if (et < C::kTokens) sx[et] = et < tile.rows ? __ldg(p.sx + (p.sx_per_row ? tile.m0 + et : 0)) : 0.0f;
       const int64_t n = tile.n0 + (CG == 2 ? static_cast<int64_t>(rank) * WROWS : 0) + q * 32 + lane;
       const int64_t at = static_cast<int64_t>(tile.e) * p.N + n;
-      const bool in = n < p.N;
+      const bool in = n < p.N && n < tile.n0 + p.tile_rows;  // lanes beyond a narrow tile hold nothing
       const float sw = in ? __ldg(p.sw + at) : 0.0f;
       const float bias = (in && p.bias) ? __ldg(p.bias + at) : 0.0f;
       const int corr = (in && p.wsum) ? zx * __ldg(p.wsum + at) : 0;
@@ -649,6 +659,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       l.m0 = tile.m0;
       l.rows = tile.rows;
       l.n = n;
+      l.in = in;
       l.sw = sw;
       l.bias = bias;
       l.corr = corr;
@@ -739,10 +750,6 @@ static Kernel kernel_for(int form, int dtype, int act) {
 static int smem_of(int form) {
   return form == kSplit16 ? smem_bytes<kSplit16>() : form == kSplit64 ? smem_bytes<kSplit64>() : smem_bytes<kPair>();
 }
-static int tokens_of(int form) {
-  return form == kSplit16 ? Cfg<kSplit16>::kTokens : form == kSplit64 ? Cfg<kSplit64>::kTokens : Cfg<kPair>::kTokens;
-}
-
 static void launch_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attrs, unsigned grid, int smem, int cluster,
                           cudaStream_t st) {
   *cfg = {};
@@ -822,7 +829,8 @@ static int choose_form(const Params& p, int64_t sms) {
 // Rows of q per tile of the pair form: 256, or fewer where that fills the last wave of tiles better.  Clocks of a tile:
 // a K block takes 2 per row of q on the tensor cores and at least 320 to bring in, the epilogue about 25 per row,
 // beside the next tile's main loop.
-static int pair_tokens(const Params& p, int64_t tiles_n, int num_kb, int64_t units) {
+static int pair_tokens(const Params& p, int num_kb, int64_t units) {
+  const int64_t tiles_n = (p.N + Cfg<kPair>::kTile - 1) / Cfg<kPair>::kTile;
   int best = 256;
   int64_t least = 0;
   for (int tokens : {256, 192, 128}) {
@@ -837,6 +845,48 @@ static int pair_tokens(const Params& p, int64_t tiles_n, int num_kb, int64_t uni
   return best;
 }
 
+struct Plan {
+  int tokens, tile_rows, cluster;  // rows of q and weight rows per tile, CTAs per tile
+  int64_t units;                   // tiles in flight
+};
+
+// Split form: CTAs per tile and weight rows per tile that give every SM an equal share of the weight's bytes.  The
+// cost is the bytes the busiest CTA streams, where a K block counts for 12 KB at least (its wait, four MMAs and commit
+// take 300 clocks whatever the rows), 24 KB for each tile's start and end and 48 KB for the hand-over between ranks
+// (each about half a microsecond at a CTA's 45 GB/s).  16 rows against [28672, 4096]: 22.8 us with 112-row tiles, 25.3
+// with 128 (two tiles for half of the CTAs, one for the rest); 1 row against [4096, 14336]: 13.8 us as four-CTA
+// clusters of 128 rows, 17.1 as pairs of 56 rows, 27.1 without a split.
+static Plan split_plan(const Params& p, int tokens, int num_kb, const DeviceInfo& info, int forced) {
+  Plan plan = {tokens, 128, 1, info.clusters[0]};
+  // groups that have rows, were they drawn evenly
+  double groups = 1.0;
+  if (p.offsets) {
+    const double empty = pow(1.0 - 1.0 / static_cast<double>(p.E), static_cast<double>(p.R));
+    groups = static_cast<double>(p.E) * (1.0 - empty);
+  }
+  const double rows = static_cast<double>(p.R) / groups;
+  const double row_tiles = groups * ceil(rows / tokens);
+  const int step = p.act == LC_ACT_SWIGLU ? 16 : 8;  // gate and up rows of a unit stay in one tile
+  double best = 0.0;
+  for (int i = 0; i < 4; ++i) {
+    const int s = 1 << i;
+    if (info.clusters[i] < 1 || num_kb < (forced ? 1 : 4) * s) break;
+    if (forced && s != forced && !(i == 0 && num_kb < forced)) continue;
+    for (int tile = 128; tile >= 48; tile -= step) {
+      const double tiles = row_tiles * static_cast<double>((p.N + tile - 1) / tile);
+      // (the number of groups that have rows is a guess: half a tile stands for the last wave)
+      const double waves = p.offsets ? tiles / info.clusters[i] + 0.5 : ceil(tiles / info.clusters[i]);
+      const double block = tile * BK > 12e3 ? tile * BK : 12e3;
+      const double cost = waves * ((num_kb + s - 1) / s * block + 24e3) + (s > 1 ? 48e3 : 0.0);
+      if (best == 0.0 || cost < 0.99 * best) {
+        best = cost;
+        plan = {tokens, tile, s, info.clusters[i]};
+      }
+    }
+  }
+  return plan;
+}
+
 static int32_t launch(const void* q, int64_t ldq, const int8_t* w, int64_t ldw, int64_t group_stride, int q_unsigned,
                       Params& p, int variant, cudaStream_t st) {
   const DeviceInfo* info = nullptr;
@@ -846,55 +896,36 @@ static int32_t launch(const void* q, int64_t ldq, const int8_t* w, int64_t ldw, 
   if (variant == 2) form = kPair;
   if (variant != 0 && variant != 2 && form == kPair) form = kSplit64;
   const bool pair = form == kPair;
-  const int forced = variant > 2 ? 1 << (variant - 3) : 0;
-  const int tile_n = pair ? 256 : 128;
-  const int64_t tiles_n = (p.N + tile_n - 1) / tile_n;
   const int num_kb = static_cast<int>((p.K + BK - 1) / BK);
-  int tokens = tokens_of(form);
-  if (pair) tokens = pair_tokens(p, tiles_n, num_kb, sms / 2);
-  p.tokens = tokens;
+  Plan plan = {256, 256, 2, sms / 2};
+  if (pair)
+    plan.tokens = pair_tokens(p, num_kb, sms / 2);
+  else
+    plan = split_plan(p, form == kSplit16 ? Cfg<kSplit16>::kTokens : Cfg<kSplit64>::kTokens, num_kb, *info,
+                      variant > 2 ? 1 << (variant - 3) : 0);
+  p.tokens = plan.tokens;
+  p.tile_rows = plan.tile_rows;
+  p.split = pair ? 1 : plan.cluster;
   CUtensorMap map_w, map_q, map_q_full;
   if (int32_t rc = encode_tensor_map_3d(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, p.K, p.N, p.E, ldw, group_stride, BK,
-                                        WROWS, CU_TENSOR_MAP_SWIZZLE_128B))
+                                        pair ? WROWS : plan.tile_rows, CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
   if (int32_t rc = encode_tensor_map_2d(&map_q, CU_TENSOR_MAP_DATA_TYPE_UINT8, q, p.K, p.R, ldq, BK,
                                         pair ? Cfg<kPair>::kBox : Cfg<kSplit64>::kBox, CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
   if (int32_t rc = encode_tensor_map_2d(&map_q_full, CU_TENSOR_MAP_DATA_TYPE_UINT8, q, p.K, p.R, ldq, BK,
-                                        pair ? tokens / 2 : tokens, CU_TENSOR_MAP_SWIZZLE_128B))
+                                        pair ? plan.tokens / 2 : plan.tokens, CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
   // kind::i8: D s32 (2) in bits [4,6); A (weight, s8 = 1) in [7,10), B (codes, s8 = 1 or u8 = 0) in [10,13); both
   // K-major; N >> 3 in [17,23) is filled in per tile; M >> 4 in [24,29)
   p.idesc = (2u << 4) | (1u << 7) | ((q_unsigned ? 0u : 1u) << 10) |
             (static_cast<uint32_t>((pair ? 256 : 128) >> 4) << 24);
-  const int64_t tiles = row_tiles(p, tokens) * tiles_n;
+  const int64_t tiles = row_tiles(p, plan.tokens) * ((p.N + plan.tile_rows - 1) / plan.tile_rows);
   if (tiles > 0x7fffffffLL) return fail(LC_ERR_UNSUPPORTED, "grouped_linear: too many tiles");
-  int cluster = 2;
-  int64_t units = sms / 2;
-  p.split = 1;
-  if (!pair) {
-    // K split: the waves of tiles over the clusters that fit, times each CTA's share of K; two K blocks of
-    // hand-over are charged per split tile
-    double best = 0.0;
-    cluster = 1;
-    units = sms;
-    for (int i = 0; i < 4; ++i) {
-      const int s = 1 << i;
-      if (info->clusters[i] < 1 || num_kb < (forced ? 1 : 4) * s) break;
-      const int64_t waves = (tiles + info->clusters[i] - 1) / info->clusters[i];
-      const double cost = static_cast<double>(waves) * ((num_kb + s - 1) / s + (s > 1 ? 2 : 0));
-      if (forced ? s == forced : i == 0 || cost < best) {
-        best = cost;
-        cluster = s;
-        units = info->clusters[i];
-      }
-    }
-    p.split = cluster;
-  }
-  if (units > tiles) units = tiles;
+  const int64_t units = plan.units < tiles ? plan.units : tiles;
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attrs[2];
-  launch_config(&cfg, attrs, static_cast<unsigned>(units * cluster), smem_of(form), cluster, st);
+  launch_config(&cfg, attrs, static_cast<unsigned>(units * plan.cluster), smem_of(form), plan.cluster, st);
   const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel_for(form, p.out_dtype, p.act), map_w, map_q, map_q_full, p);
   if (err != cudaSuccess) return fail(LC_ERR_CUDA, "grouped_linear: %s", cudaGetErrorString(err));
   return check_launch("grouped_linear");
