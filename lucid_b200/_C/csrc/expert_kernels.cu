@@ -43,8 +43,11 @@ struct Vec16 {
 // A logit of -inf or NaN is never chosen and carries no weight (masked experts, padded tokens); what is not
 // chosen has expert -1, position -1 and weight 0.  +inf shares the weight with the other +inf of its row.
 //
-// One warp per token: the row sits in registers (EPL values per lane), each of the top_k rounds is a local
-// maximum and two warp-wide integer reductions (order-preserving bits of the value, then the lowest index).
+// One warp per token: lane l holds the EPL values l*EPL .. l*EPL + EPL-1 in registers and their maximum.  A round is
+// one warp-wide integer maximum (order-preserving bits of the value) and a vote: of several lanes with the largest
+// value the lowest has the lowest expert, and that lane moves on to its next one.  Up to four values a lane are
+// sorted first, so that moving on is a shift (16384 x 128, 8 of them: 538 -> TODO instructions a token, which is what
+// the kernel is bound by); more are searched.
 // A warp walks a contiguous run of tokens and counts its choices per expert in shared memory; a choice's
 // count is its rank inside the run.  Small batches (one CTA) finish in the same kernel; otherwise each CTA
 // leaves its counts and its ranks, and the second kernel adds what precedes them.  Every sum is an integer
@@ -72,7 +75,8 @@ struct RouteParams {
   int32_t* positions;  // [tokens, top_k]
   int32_t* offsets;    // [experts + 1]
   int32_t* counts;     // [CTAs, experts], several CTAs only
-  int run;             // tokens per warp
+  int per_cta, run;    // tokens per CTA and per warp
+  int vec;             // rows may be read in vectors
 };
 
 // inclusive sum over the block of one int per thread; `tmp` holds 32 ints
@@ -99,6 +103,29 @@ __device__ __forceinline__ int block_scan(int v, int* tmp) {
   return v + (warp ? tmp[warp - 1] : 0);
 }
 
+template <typename T, int EPL>
+__device__ __forceinline__ void load_row(const T* row, int E, int lane, int vec, T (&v)[EPL]) {
+  if (vec) {  // E is 32 * EPL and rows start on a boundary of the lane's bytes
+    constexpr int kBytes = EPL * sizeof(T) < 16 ? EPL * sizeof(T) : 16, kPer = kBytes / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < EPL; i += kPer) {
+      const T* src = row + lane * EPL + i;
+      if constexpr (kBytes == 16)
+        *reinterpret_cast<uint4*>(v + i) = __ldg(reinterpret_cast<const uint4*>(src));
+      else if constexpr (kBytes == 8)
+        *reinterpret_cast<uint2*>(v + i) = __ldg(reinterpret_cast<const uint2*>(src));
+      else if constexpr (kBytes == 4)
+        *reinterpret_cast<uint32_t*>(v + i) = __ldg(reinterpret_cast<const uint32_t*>(src));
+      else
+        v[i] = src[0];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+      if (lane * EPL + i < E) v[i] = row[lane * EPL + i];
+  }
+}
+
 template <typename T, int EPL, bool ONE_CTA>
 __global__ void __launch_bounds__(1024) route_kernel(const RouteParams p) {
   extern __shared__ int s_counts[];  // [warps][experts]; one CTA: then [experts] bases
@@ -111,55 +138,92 @@ __global__ void __launch_bounds__(1024) route_kernel(const RouteParams p) {
   pdl_wait();
   __syncthreads();
 
-  const int64_t first = (static_cast<int64_t>(blockIdx.x) * warps + warp) * p.run;
-  const int64_t last = first + p.run < p.tokens ? first + p.run : p.tokens;
+  const int64_t begin = static_cast<int64_t>(blockIdx.x) * p.per_cta;
+  const int64_t end = begin + p.per_cta < p.tokens ? begin + p.per_cta : p.tokens;
+  const int64_t first = begin + warp * p.run;
+  const int64_t last = first + p.run < end ? first + p.run : end;
+  T next[EPL];
+  if (first < last) load_row<T, EPL>(static_cast<const T*>(p.logits) + first * p.ld, E, lane, p.vec, next);
   for (int64_t t = first; t < last; ++t) {
-    const T* row = static_cast<const T*>(p.logits) + t * p.ld;
-    uint32_t key[EPL];
+    uint32_t key[EPL], top = 0;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      const int e = i * 32 + lane;
-      key[i] = e < E ? order_bits(to_float<T>(row[e])) : 0u;
+      key[i] = lane * EPL + i < E ? order_bits(to_float<T>(next[i])) : 0u;
+      top = max(top, key[i]);
     }
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) top = max(top, key[i]);
+    if (t + 1 < last) load_row<T, EPL>(static_cast<const T*>(p.logits) + (t + 1) * p.ld, E, lane, p.vec, next);
+    uint32_t mine_max = top;
     top = __reduce_max_sync(0xffffffffu, top);
     const float largest = order_value(top);
-    // exp(v - largest); with an infinite largest value 1 for those equal to it and 0 for the rest
     const bool finite = largest < INFINITY;
+    // exp(v - largest); with an infinite largest value 1 for those equal to it and 0 for the rest
+    auto mass = [&](uint32_t k) {
+      return k == 0u ? 0.0f : finite ? expf(order_value(k) - largest) : (k == top ? 1.0f : 0.0f);
+    };
     float total = 0.0f;
-    if (!p.renormalize && top) {
+    if (!p.renormalize) {
 #pragma unroll
-      for (int i = 0; i < EPL; ++i)
-        if (key[i]) total += finite ? expf(order_value(key[i]) - largest) : (key[i] == top ? 1.0f : 0.0f);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+      for (int i = 0; i < EPL; ++i) total += mass(key[i]);
     }
     // lane j keeps the j-th choice
-    float my_p = 0.0f;
+    uint32_t my_key = 0, best = top;
     int my_e = -1;
-    uint32_t best = top;
-    for (int j = 0; j < K && best; ++j) {
-      uint32_t at = 0xffffffffu;
+    if constexpr (EPL <= 4) {
+      // descending, equal values in the order of their experts; two bits per value say where it came from
+      uint32_t from = 0xe4u;  // 3, 2, 1, 0
+      auto order = [&](int i) {  // values i and i + 1
+        const bool swap = key[i + 1] > key[i];
+        const uint32_t hi = max(key[i], key[i + 1]), lo = min(key[i], key[i + 1]);
+        key[i] = hi;
+        key[i + 1] = lo;
+        const uint32_t bits = ((from >> 2 * i) ^ (from >> 2 * (i + 1))) & 3u;
+        if (swap) from ^= bits << 2 * i | bits << 2 * (i + 1);
+      };
 #pragma unroll
-      for (int i = EPL - 1; i >= 0; --i)
-        if (key[i] == best) at = i * 32 + lane;
-      at = __reduce_min_sync(0xffffffffu, at);
-      const float pr = finite ? expf(order_value(best) - largest) : (best == top ? 1.0f : 0.0f);
-      if (p.renormalize) total += pr;
-      if (lane == j) {
-        my_p = pr;
-        my_e = static_cast<int>(at);
-      }
-      uint32_t next = 0;
+      for (int n = EPL - 1; n > 0; --n)
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) {
-        if (i * 32 + lane == static_cast<int>(at)) key[i] = 0u;
-        next = max(next, key[i]);
+        for (int i = 0; i < n; ++i) order(i);
+      for (int j = 0; j < K && best; ++j) {
+        const int winner = __ffs(__ballot_sync(0xffffffffu, key[0] == best)) - 1;
+        const int e = __shfl_sync(0xffffffffu, lane * EPL + static_cast<int>(from & 3u), winner);
+        if (lane == j) {
+          my_key = best;
+          my_e = e;
+        }
+        if (lane == winner) {
+#pragma unroll
+          for (int i = 0; i < EPL; ++i) key[i] = i + 1 < EPL ? key[i + 1] : 0u;
+          from >>= 2;
+        }
+        best = __reduce_max_sync(0xffffffffu, key[0]);
       }
-      best = __reduce_max_sync(0xffffffffu, next);
+    } else {
+      for (int j = 0; j < K && best; ++j) {
+        const int winner = __ffs(__ballot_sync(0xffffffffu, mine_max == best)) - 1;
+        int at = 0;
+        if (lane == winner) {
+#pragma unroll
+          for (int i = EPL - 1; i >= 0; --i)
+            if (key[i] == best) at = i;
+          mine_max = 0;
+#pragma unroll
+          for (int i = 0; i < EPL; ++i) {
+            if (i == at) key[i] = 0u;
+            mine_max = max(mine_max, key[i]);
+          }
+        }
+        at = __shfl_sync(0xffffffffu, at, winner);
+        if (lane == j) {
+          my_key = best;
+          my_e = winner * EPL + at;
+        }
+        best = __reduce_max_sync(0xffffffffu, mine_max);
+      }
     }
+    const float my_p = mass(my_key);
+    if (p.renormalize) total = my_p;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     if (lane < K) {
       int rank = -1;
       if (my_e >= 0) rank = mine[my_e]++;  // a token's choices are distinct experts: no two lanes meet
@@ -249,10 +313,11 @@ __global__ void __launch_bounds__(1024) route_place_kernel(const RouteParams p, 
 
 constexpr int kRouteWarps = 32;
 constexpr int64_t kRouteOneCta = 128;  // tokens that one CTA routes and places in one kernel
-constexpr int64_t kRouteCtas = 128;    // CTAs of a larger batch: tokens per warp grow beyond that
+constexpr int64_t kRouteCtas = 148;    // most CTAs of a larger batch: one for each SM
 
-int64_t route_run(int64_t tokens) {  // tokens per warp
-  return (tokens + kRouteCtas * kRouteWarps - 1) / (kRouteCtas * kRouteWarps);
+int64_t route_per_cta(int64_t tokens) {  // at least one token per warp
+  const int64_t n = (tokens + kRouteCtas - 1) / kRouteCtas;
+  return n > kRouteWarps ? n : kRouteWarps;
 }
 
 template <typename T, int EPL>
@@ -262,6 +327,8 @@ cudaError_t launch_route(RouteParams p, cudaStream_t st) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   const int one = p.tokens <= kRouteOneCta;
+  constexpr int kLaneBytes = EPL * sizeof(T) < 16 ? EPL * sizeof(T) : 16;
+  p.vec = p.experts == 32 * EPL && aligned(p.logits, kLaneBytes) && (p.ld * sizeof(T)) % kLaneBytes == 0;
   std::call_once(flags[dev][one], [dev, one]() {
     const int bytes = (kRouteWarps + 1) * EPL * 32 * 4;
     results[dev][one] =
@@ -270,12 +337,10 @@ cudaError_t launch_route(RouteParams p, cudaStream_t st) {
   });
   if (results[dev][one] != cudaSuccess) return results[dev][one];
   const size_t smem = static_cast<size_t>(kRouteWarps + 1) * p.experts * 4;
-  if (one) {
-    p.run = static_cast<int>((p.tokens + kRouteWarps - 1) / kRouteWarps);
-    return launch_overlapped(route_kernel<T, EPL, true>, dim3(1), dim3(1024), smem, st, p);
-  }
-  p.run = static_cast<int>(route_run(p.tokens));
-  const int64_t per_cta = static_cast<int64_t>(kRouteWarps) * p.run;
+  const int64_t per_cta = one ? p.tokens : route_per_cta(p.tokens);
+  p.per_cta = static_cast<int>(per_cta);
+  p.run = static_cast<int>((per_cta + kRouteWarps - 1) / kRouteWarps);
+  if (one) return launch_overlapped(route_kernel<T, EPL, true>, dim3(1), dim3(1024), smem, st, p);
   const int ctas = static_cast<int>((p.tokens + per_cta - 1) / per_cta);
   cudaError_t err = launch_overlapped(route_kernel<T, EPL, false>, dim3(ctas), dim3(1024), smem, st, p);
   if (err != cudaSuccess) return err;
@@ -543,7 +608,7 @@ using namespace lc;
 
 extern "C" int64_t lc_route_experts_workspace_bytes(int64_t tokens, int64_t experts) {
   if (tokens <= kRouteOneCta || experts <= 0) return 0;
-  const int64_t per_cta = kRouteWarps * route_run(tokens);
+  const int64_t per_cta = route_per_cta(tokens);
   return (tokens + per_cta - 1) / per_cta * experts * 4;
 }
 

@@ -46,35 +46,28 @@ constexpr int EPI_WARPS = 8;
 constexpr int EPI_THREADS = EPI_WARPS * 32;
 constexpr int MAX_GROUPS = 1024;
 
-// kTokens: rows of q per tile; kStep: granularity of the instruction's N; kBox: rows of q per TMA box of a tile
-// that is not full; kRed: bytes of rank 0's buffer for the other ranks' partial sums, [column][lane]
-template <int FORM>
+// kTokens: most rows of q per tile; kStep: granularity of the instruction's N; kBox: rows of q per TMA box of a tile
+// that is not full; kRing: bytes of the operand ring (its stages are 16 KB of weights and the tile's codes); kRed:
+// bytes of rank 0's buffer for the other ranks' partial sums, [column][lane]
+template <int CG>
 struct Cfg;
-constexpr int kSplit16 = 0, kSplit64 = 1, kPair = 2;
 template <>
-struct Cfg<kSplit16> {
-  static constexpr int kCtas = 1, kTile = 128, kTokens = 16, kStep = 16, kBox = 16, kStages = 9;
-  static constexpr int kBBytes = kTokens * BK, kRed = kTokens * WROWS * 4;
+struct Cfg<1> {
+  static constexpr int kTokens = 64, kStep = 16, kBox = 16;
+  static constexpr int kRing = 7 * (A_BYTES + kTokens * BK), kRed = kTokens * WROWS * 4;
 };
 template <>
-struct Cfg<kSplit64> {
-  static constexpr int kCtas = 1, kTile = 128, kTokens = 64, kStep = 16, kBox = 16, kStages = 7;
-  static constexpr int kBBytes = kTokens * BK, kRed = kTokens * WROWS * 4;
+struct Cfg<2> {
+  static constexpr int kTokens = 256, kStep = 32, kBox = 32;
+  static constexpr int kRing = 6 * (A_BYTES + kTokens / 2 * BK), kRed = 0;
 };
-template <>
-struct Cfg<kPair> {
-  static constexpr int kCtas = 2, kTile = 256, kTokens = 256, kStep = 32, kBox = 32, kStages = 6;
-  static constexpr int kBBytes = (kTokens / 2) * BK, kRed = 0;
-};
-template <int FORM>
-__host__ __device__ constexpr int stage_bytes() { return A_BYTES + Cfg<FORM>::kBBytes; }
-template <int FORM>
+constexpr int MAX_STAGES = 12;
+template <int CG>
 __host__ __device__ constexpr int smem_bytes() {
-  return 1024 + Cfg<FORM>::kStages * stage_bytes<FORM>() + 256 + Cfg<FORM>::kRed + 2 * Cfg<FORM>::kTokens * 4 +
-         2 * (MAX_GROUPS + 1) * 4;
+  return 1024 + Cfg<CG>::kRing + 256 + Cfg<CG>::kRed + 2 * Cfg<CG>::kTokens * 4 + 2 * (MAX_GROUPS + 1) * 4;
 }
-static_assert(smem_bytes<kSplit16>() <= 232448 && smem_bytes<kSplit64>() <= 232448 && smem_bytes<kPair>() <= 232448,
-              "shared memory of a CTA");
+static_assert(smem_bytes<1>() <= 232448 && smem_bytes<2>() <= 232448, "shared memory of a CTA");
+static_assert(2 * MAX_STAGES * 8 + 6 * 8 <= 256 && MAX_STAGES + 3 <= 31, "barrier area; a lane sets each pair up");
 
 enum : int { ST_PRODUCER = 1, ST_MMA = 2, ST_EPILOGUE = 3 };
 
@@ -97,7 +90,8 @@ struct Params {
   int32_t* status;
   int wait_test;
   int tokens;               // rows of q per tile, at most the form's kTokens
-  int tile_rows;            // weight rows per tile: the form's kTile, or fewer (a multiple of 8) in the split form
+  int tile_rows;            // weight rows per tile: 128 (256 in a pair) or fewer, a multiple of 8 for each CTA
+  int stages, stage_bytes;  // of the operand ring
   int split;                // CTAs of a cluster that share a tile's K (CG == 1)
   int early_weights;        // the weight and offsets were complete before the previous kernel began
   uint32_t idesc;           // instruction descriptor without its N field
@@ -353,21 +347,19 @@ __device__ __forceinline__ void drain(const Params& p, const Lane& l) {
   }
 }
 
-template <int FORM, typename T, int ACT>
+template <int CG, typename T, int ACT>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_q,
                       const __grid_constant__ CUtensorMap tmap_q_full, const Params p) {
-  using C = Cfg<FORM>;
-  constexpr int CG = C::kCtas;
-  constexpr int STAGES = C::kStages, STAGE_BYTES = stage_bytes<FORM>();
-  constexpr int TMEM_COLS = 2 * C::kTokens;  // 32, 128 or 512
-  static_assert(2 * STAGES * 8 + 6 * 8 <= 256, "barrier area");
+  using C = Cfg<CG>;
+  const int stages = p.stages, stage_bytes = p.stage_bytes;
+  constexpr int TMEM_COLS = 2 * C::kTokens;  // 128 or 512
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint32_t s_tmem_base;
 
   pdl_launch_dependents();
   const uint32_t tiles_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t bar_base = tiles_base + STAGES * STAGE_BYTES;
+  const uint32_t bar_base = tiles_base + C::kRing;
   const uint32_t red_base = bar_base + 256;
   uint8_t* const after = smem_raw + (red_base - smem_u32(smem_raw));
   int* const s_red = reinterpret_cast<int*>(after);
@@ -375,10 +367,10 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   int* const s_off = reinterpret_cast<int*>(s_sx + 2 * C::kTokens);
   int* const s_start = s_off + (MAX_GROUPS + 1);
   auto full_bar = [&](int s) { return bar_base + 8u * s; };
-  auto empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
-  auto acc_full_bar = [&](int s) { return bar_base + 8u * (2 * STAGES + s); };
-  auto acc_empty_bar = [&](int s) { return bar_base + 8u * (2 * STAGES + 2 + s); };
-  const uint32_t part_bar = bar_base + 8u * (2 * STAGES + 4);  // rank 0: the other ranks' sums have been added
+  auto empty_bar = [&](int s) { return bar_base + 8u * (MAX_STAGES + s); };
+  auto acc_full_bar = [&](int s) { return bar_base + 8u * (2 * MAX_STAGES + s); };
+  auto acc_empty_bar = [&](int s) { return bar_base + 8u * (2 * MAX_STAGES + 2 + s); };
+  const uint32_t part_bar = bar_base + 8u * (2 * MAX_STAGES + 4);  // rank 0: the other ranks' sums have been added
   const uint32_t free_bar = part_bar + 8u;                     // other ranks: rank 0's buffer is zero again
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -397,13 +389,13 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   uint32_t armed = 0, armed_parity = 0;  // producer: stages with copies in flight, one bit each
   int ahead = 0;                         // producer: stages whose weights have been requested
   if (warp == 0) {
-    if (lane < STAGES) {
+    if (lane < MAX_STAGES) {
       mbar_init(full_bar(lane), 1);
       mbar_init(empty_bar(lane), 1);
-    } else if (lane < STAGES + 2) {
-      mbar_init(acc_full_bar(lane - STAGES), 1);
-      mbar_init(acc_empty_bar(lane - STAGES), CG * EPI_WARPS);
-    } else if (lane == STAGES + 2) {
+    } else if (lane < MAX_STAGES + 2) {
+      mbar_init(acc_full_bar(lane - MAX_STAGES), 1);
+      mbar_init(acc_empty_bar(lane - MAX_STAGES), CG * EPI_WARPS);
+    } else if (lane == MAX_STAGES + 2) {
       mbar_init(part_bar, 1);
       mbar_init(free_bar, EPI_WARPS);
     } else if (lane == 31) {
@@ -454,11 +446,11 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       const Tile tile = walk.at(unit);
       const int n0 = static_cast<int>(tile.n0), boxes = (tile.rows + C::kBox - 1) / C::kBox;
       const uint32_t bytes = static_cast<uint32_t>((p.tile_rows + boxes * C::kBox) * BK);
-      ahead = min(STAGES, kb1 - kb0);
+      ahead = min(stages, kb1 - kb0);
       if (elect_one())
         for (int s = 0; s < ahead; ++s) {
           mbar_expect_tx(full_bar(s), bytes);
-          tma_load_3d(tiles_base + s * STAGE_BYTES, &tmap_w, (kb0 + s) * BK, n0, tile.e, full_bar(s));
+          tma_load_3d(tiles_base + s * stage_bytes, &tmap_w, (kb0 + s) * BK, n0, tile.e, full_bar(s));
         }
       __syncwarp();
       armed = (1u << ahead) - 1;
@@ -505,11 +497,11 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       const bool full = mine == p.tokens / CG;  // one box; else as many of kBox rows as it takes
       const int boxes = (mine + C::kBox - 1) / C::kBox;
       const uint32_t bytes = static_cast<uint32_t>((p.tile_rows + CG * (full ? mine : boxes * C::kBox)) * BK);
-      const int n0 = static_cast<int>(tile.n0) + (CG == 2 ? static_cast<int>(rank) * WROWS : 0);
+      const int n0 = static_cast<int>(tile.n0) + (CG == 2 ? static_cast<int>(rank) * (p.tile_rows / 2) : 0);
       const int m0 = tile.m0 + (CG == 2 ? static_cast<int>(rank) * mine : 0);
       const int e = tile.e;
       auto load_q = [&](int s, int kb) {
-        const uint32_t dst = tiles_base + s * STAGE_BYTES + A_BYTES;
+        const uint32_t dst = tiles_base + s * stage_bytes + A_BYTES;
         if (full) {
           if constexpr (CG == 2)
             tma_load_2d_pair(dst, &tmap_q_full, kb * BK, m0, map_to_cta(full_bar(s), 0));
@@ -530,8 +522,8 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
           for (int s = 0; s < ahead; ++s) load_q(s, kb0 + s);
         __syncwarp();
         kb = kb0 + ahead;
-        stage = ahead % STAGES;
-        phase = ahead == STAGES ? 1u : 0u;
+        stage = ahead % stages;
+        phase = ahead == stages ? 1u : 0u;
       }
       for (; kb < kb1; ++kb) {
         if (!__all_sync(0xffffffffu, mbar_wait(empty_bar(stage), phase ^ 1u, budget))) {
@@ -540,7 +532,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
           break;
         }
         if (elect_one()) {
-          const uint32_t dst = tiles_base + stage * STAGE_BYTES;
+          const uint32_t dst = tiles_base + stage * stage_bytes;
           if (CG == 1 || leader) mbar_expect_tx(full_bar(stage), bytes);
           if constexpr (CG == 2)
             tma_load_3d_pair(dst, &tmap_w, kb * BK, n0, e, map_to_cta(full_bar(stage), 0));
@@ -553,14 +545,14 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
           armed |= 1u << stage;
           armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
         }
-        if (++stage == STAGES) {
+        if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
         }
       }
     }
     // do not leave while a bulk copy may still be landing (a pair's leader counts the bytes of both CTAs)
-    for (int s = 0; s < STAGES; ++s)
+    for (int s = 0; s < stages; ++s)
       if (armed >> s & 1) mbar_wait(full_bar(s), armed_parity >> s & 1);
     __syncwarp();
   } else if (warp == 1) {
@@ -589,7 +581,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
           }
           tc_fence_after();
           if (elect_one()) {
-            const uint32_t src = tiles_base + stage * STAGE_BYTES;
+            const uint32_t src = tiles_base + stage * stage_bytes;
             const uint64_t w_desc = make_smem_desc(src), q_desc = make_smem_desc(src + A_BYTES);
 #pragma unroll
             for (int j = 0; j < BK / UMMA_K; ++j) {
@@ -606,7 +598,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
               tc_commit(empty_bar(stage));
           }
           __syncwarp();
-          if (++stage == STAGES) {
+          if (++stage == stages) {
             stage = 0;
             phase ^= 1u;
           }
@@ -634,9 +626,10 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       const int as = it & 1;
       float* const sx = s_sx + as * C::kTokens;
       if (et < C::kTokens) sx[et] = et < tile.rows ? __ldg(p.sx + (p.sx_per_row ? tile.m0 + et : 0)) : 0.0f;
-      const int64_t n = tile.n0 + (CG == 2 ? static_cast<int64_t>(rank) * WROWS : 0) + q * 32 + lane;
+      const int cta_rows = p.tile_rows / CG;
+      const int64_t n = tile.n0 + (CG == 2 ? static_cast<int64_t>(rank) * cta_rows : 0) + q * 32 + lane;
       const int64_t at = static_cast<int64_t>(tile.e) * p.N + n;
-      const bool in = n < p.N && n < tile.n0 + p.tile_rows;  // lanes beyond a narrow tile hold nothing
+      const bool in = n < p.N && q * 32 + lane < cta_rows;  // lanes beyond a narrow tile hold nothing
       const float sw = in ? __ldg(p.sw + at) : 0.0f;
       const float bias = (in && p.bias) ? __ldg(p.bias + at) : 0.0f;
       const int corr = (in && p.wsum) ? zx * __ldg(p.wsum + at) : 0;
@@ -724,32 +717,24 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
 // ---- host side -------------------------------------------------------------------------------
 using Kernel = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, Params);
 
-template <int FORM, typename T>
+template <int CG, typename T>
 static Kernel kernel_for(int act) {
   switch (act) {
-    case LC_ACT_RELU: return grouped_linear_kernel<FORM, T, LC_ACT_RELU>;
-    case LC_ACT_GELU: return grouped_linear_kernel<FORM, T, LC_ACT_GELU>;
-    case LC_ACT_GELU_TANH: return grouped_linear_kernel<FORM, T, LC_ACT_GELU_TANH>;
-    case LC_ACT_SILU: return grouped_linear_kernel<FORM, T, LC_ACT_SILU>;
-    case LC_ACT_SWIGLU: return grouped_linear_kernel<FORM, T, LC_ACT_SWIGLU>;
-    default: return grouped_linear_kernel<FORM, T, LC_ACT_NONE>;
+    case LC_ACT_RELU: return grouped_linear_kernel<CG, T, LC_ACT_RELU>;
+    case LC_ACT_GELU: return grouped_linear_kernel<CG, T, LC_ACT_GELU>;
+    case LC_ACT_GELU_TANH: return grouped_linear_kernel<CG, T, LC_ACT_GELU_TANH>;
+    case LC_ACT_SILU: return grouped_linear_kernel<CG, T, LC_ACT_SILU>;
+    case LC_ACT_SWIGLU: return grouped_linear_kernel<CG, T, LC_ACT_SWIGLU>;
+    default: return grouped_linear_kernel<CG, T, LC_ACT_NONE>;
   }
 }
-template <int FORM>
+template <int CG>
 static Kernel kernel_for(int dtype, int act) {
-  return dtype == LC_F32    ? kernel_for<FORM, float>(act)
-         : dtype == LC_BF16 ? kernel_for<FORM, __nv_bfloat16>(act)
-                            : kernel_for<FORM, __half>(act);
+  return dtype == LC_F32    ? kernel_for<CG, float>(act)
+         : dtype == LC_BF16 ? kernel_for<CG, __nv_bfloat16>(act)
+                            : kernel_for<CG, __half>(act);
 }
 
-static Kernel kernel_for(int form, int dtype, int act) {
-  return form == kSplit16   ? kernel_for<kSplit16>(dtype, act)
-         : form == kSplit64 ? kernel_for<kSplit64>(dtype, act)
-                            : kernel_for<kPair>(dtype, act);
-}
-static int smem_of(int form) {
-  return form == kSplit16 ? smem_bytes<kSplit16>() : form == kSplit64 ? smem_bytes<kSplit64>() : smem_bytes<kPair>();
-}
 static void launch_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attrs, unsigned grid, int smem, int cluster,
                           cudaStream_t st) {
   *cfg = {};
@@ -783,18 +768,19 @@ static int32_t device_info(const DeviceInfo** out) {
     DeviceInfo& info = infos[dev];
     info.err = cudaSuccess;
     for (int dtype : {LC_F32, LC_BF16, LC_F16})
-      for (int act = LC_ACT_NONE; act <= LC_ACT_SWIGLU; ++act)
-        for (int form : {kSplit16, kSplit64, kPair})
-          if (info.err == cudaSuccess)
-            info.err = cudaFuncSetAttribute(kernel_for(form, dtype, act), cudaFuncAttributeMaxDynamicSharedMemorySize, smem_of(form));
+      for (int act = LC_ACT_NONE; act <= LC_ACT_SWIGLU && info.err == cudaSuccess; ++act) {
+        info.err = cudaFuncSetAttribute(kernel_for<1>(dtype, act), cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<1>());
+        if (info.err == cudaSuccess)
+          info.err = cudaFuncSetAttribute(kernel_for<2>(dtype, act), cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<2>());
+      }
     const int sms = sm_count();
     for (int i = 0; i < 4 && info.err == cudaSuccess; ++i) {
       cudaLaunchConfig_t cfg;
       cudaLaunchAttribute attrs[2];
-      launch_config(&cfg, attrs, static_cast<unsigned>(sms / (1 << i) << i), smem_of(kSplit64), 1 << i, nullptr);
+      launch_config(&cfg, attrs, static_cast<unsigned>(sms / (1 << i) << i), smem_bytes<1>(), 1 << i, nullptr);
       cfg.numAttrs = 1;
       int n = 0;
-      if (cudaOccupancyMaxActiveClusters(&n, kernel_for(kSplit64, LC_F32, LC_ACT_NONE), &cfg) != cudaSuccess) {
+      if (cudaOccupancyMaxActiveClusters(&n, kernel_for<1>(LC_F32, LC_ACT_NONE), &cfg) != cudaSuccess) {
         cudaGetLastError();
         n = i == 0 ? sms : 0;
       }
@@ -813,75 +799,60 @@ static int64_t row_tiles(const Params& p, int tokens) {
   return (p.R - groups) / tokens + groups;
 }
 
-// Form by the rows a group has on average (all that is known on the host).  Above 64 rows the pair's 256 x 256 tiles
-// win once they occupy half of the machine; with fewer of them the narrow tiles spread further ([4096, 4096] weight:
-// 128 rows 18.6 against 20.4 us, 256 rows 21.3 / 22.5, 512 rows 32.8 / 23.3, launch and timing overhead of 7 us
-// included).  Up to 16 rows the smaller code tiles leave room for four more stages of weights in flight.
-static int choose_form(const Params& p, int64_t sms) {
-  if (p.R > 64 * static_cast<int64_t>(p.E)) {
-    const int64_t tiles = row_tiles(p, Cfg<kPair>::kTokens) * ((p.N + 255) / 256);
-    return p.R > 256 * static_cast<int64_t>(p.E) || tiles >= sms / 4 ? kPair : kSplit64;
-  }
-  const int64_t rows = p.offsets ? 2 * p.R : p.R;  // groups differ in size
-  return rows <= 16 * static_cast<int64_t>(p.E) ? kSplit16 : kSplit64;
-}
-
-// Rows of q per tile of the pair form: 256, or fewer where that fills the last wave of tiles better.  Clocks of a tile:
-// a K block takes 2 per row of q on the tensor cores and at least 320 to bring in, the epilogue about 25 per row,
-// beside the next tile's main loop.
-static int pair_tokens(const Params& p, int num_kb, int64_t units) {
-  const int64_t tiles_n = (p.N + Cfg<kPair>::kTile - 1) / Cfg<kPair>::kTile;
-  int best = 256;
-  int64_t least = 0;
-  for (int tokens : {256, 192, 128}) {
-    const int64_t waves = (row_tiles(p, tokens) * tiles_n + units - 1) / units;
-    const int64_t loop = static_cast<int64_t>(num_kb) * (2 * tokens > 320 ? 2 * tokens : 320), drain = 25 * tokens;
-    const int64_t cost = waves * (loop > drain ? loop : drain) + (loop < drain ? loop : drain);
-    if (tokens == 256 || cost < least - least / 32) {
-      least = cost;
-      best = tokens;
-    }
-  }
-  return best;
-}
-
 struct Plan {
-  int tokens, tile_rows, cluster;  // rows of q and weight rows per tile, CTAs per tile
-  int64_t units;                   // tiles in flight
+  int ctas, tokens, tile_rows, split;  // CTAs of an MMA (1 or 2), rows of q and weight rows per tile, CTAs along K
+  int64_t units;                       // tiles in flight
 };
 
-// Split form: CTAs per tile and weight rows per tile that give every SM an equal share of the weight's bytes.  The
-// cost is the bytes the busiest CTA streams, where a K block counts for 12 KB at least (its wait, four MMAs and commit
-// take 300 clocks whatever the rows), 24 KB for each tile's start and end and 48 KB for the hand-over between ranks
-// (each about half a microsecond at a CTA's 45 GB/s).  16 rows against [28672, 4096]: 22.8 us with 112-row tiles, 25.3
-// with 128 (two tiles for half of the CTAs, one for the rest); 1 row against [4096, 14336]: 13.8 us as four-CTA
-// clusters of 128 rows, 17.1 as pairs of 56 rows, 27.1 without a split.
-static Plan split_plan(const Params& p, int tokens, int num_kb, const DeviceInfo& info, int forced) {
-  Plan plan = {tokens, 128, 1, info.clusters[0]};
-  // groups that have rows, were they drawn evenly
-  double groups = 1.0;
+// Form and tile sizes, by the clocks that the busiest CTA is expected to take.  A K block costs the larger of its
+// MMAs (2 clocks per row of q in a pair, 1 else), of bringing it in (64 bytes a clock, 40 for weights used once) and of
+// 300 clocks for a wait, four MMAs and a commit; the epilogue takes 25 clocks per row of q and runs beside the next tile's main loop; a tile
+// costs 600 clocks more, and 1500 where K is split.  Tiles come in waves over the CTAs there are; the number of groups
+// that have rows is not known on the host, so that half a tile stands for the last wave of a grouped product.
+// Measured, product alone, weights from HBM:
+//   16 rows,  [28672, 4096] SwiGLU   pair, 112 rows a CTA 22.8 us; pair, 128 24.0; one CTA, 112 23.7, 128 24.8
+//   16 rows,  [4096, 14336]          K over 4 CTAs 14.4 us; over 2 18.0; over 8 18.0; over 4 with 112 rows 19.4
+//   333 rows, [1232, 1008]           pair, 64 rows of q a tile 5.7 us, 128 6.1 to 6.8, 192 7.1 to 7.9
+//   256 rows, [4096, 4096]           pair, 64 rows of q 11.0 us, 128 11.5, 256 15.4; one CTA, 64 12.5
+//   64 groups of 84 rows, [2048, 1408]   pair, 128 rows of q 38.5 us, 64 50.2; one CTA, 64 54.2
+//   32 groups of 8 rows, [4096, 4096]    pair 80.8 us, one CTA 83.3
+static Plan make_plan(const Params& p, const DeviceInfo& info, int64_t sms, int variant) {
+  const int num_kb = static_cast<int>((p.K + BK - 1) / BK);
+  const int forced = variant > 2 ? 1 << (variant - 3) : 0;
+  double groups = 1.0;  // that have rows, were these drawn evenly
   if (p.offsets) {
     const double empty = pow(1.0 - 1.0 / static_cast<double>(p.E), static_cast<double>(p.R));
     groups = static_cast<double>(p.E) * (1.0 - empty);
   }
   const double rows = static_cast<double>(p.R) / groups;
-  const double row_tiles = groups * ceil(rows / tokens);
   const int step = p.act == LC_ACT_SWIGLU ? 16 : 8;  // gate and up rows of a unit stay in one tile
+  Plan plan = {2, 256, 256, 1, sms / 2};
   double best = 0.0;
-  for (int i = 0; i < 4; ++i) {
-    const int s = 1 << i;
-    if (info.clusters[i] < 1 || num_kb < (forced ? 1 : 4) * s) break;
-    if (forced && s != forced && !(i == 0 && num_kb < forced)) continue;
-    for (int tile = 128; tile >= 48; tile -= step) {
-      const double tiles = row_tiles * static_cast<double>((p.N + tile - 1) / tile);
-      // (the number of groups that have rows is a guess: half a tile stands for the last wave)
-      const double waves = p.offsets ? tiles / info.clusters[i] + 0.5 : ceil(tiles / info.clusters[i]);
-      const double block = tile * BK > 12e3 ? tile * BK : 12e3;
-      const double cost = waves * ((num_kb + s - 1) / s * block + 24e3) + (s > 1 ? 48e3 : 0.0);
-      if (best == 0.0 || cost < 0.99 * best) {
+  auto consider = [&](int ctas, int split, int64_t units, int tokens) {
+    const double row_tiles = groups * ceil(rows / tokens), cols = rows < tokens ? rows : tokens;
+    for (int cta_rows = 128; cta_rows >= 48; cta_rows -= step) {
+      const double tiles = row_tiles * static_cast<double>((p.N + ctas * cta_rows - 1) / (ctas * cta_rows));
+      const double waves = p.offsets ? tiles / units + 0.5 : ceil(tiles / units);
+      // (weights that only one row tile reads come from HBM, of which a CTA gets less than of the L2)
+      const double load = cta_rows * BK / (rows <= tokens ? 40.0 : 64.0) + cols / ctas * BK / 64.0;
+      double block = ctas * cols > 300.0 ? ctas * cols : 300.0;
+      if (load > block) block = load;
+      const double loop = (num_kb + split - 1) / split * block, drain = 25.0 * cols;
+      const double cost = waves * ((loop > drain ? loop : drain) + (split > 1 ? 2100.0 : 600.0)) + (loop > drain ? drain : loop);
+      if (best == 0.0 || cost < 0.98 * best) {
         best = cost;
-        plan = {tokens, tile, s, info.clusters[i]};
+        plan = {ctas, tokens, ctas * cta_rows, split, units};
       }
+    }
+  };
+  if (variant == 0 || variant == 2)
+    for (int tokens : {64, 128, 192, 256}) consider(2, 1, sms / 2, tokens);
+  if (variant != 2) {
+    for (int i = 0; i < 4; ++i) {
+      const int split = 1 << i;
+      if (info.clusters[i] < 1 || num_kb < (forced ? 1 : 4) * split) break;
+      if (forced && split != forced && !(i == 0 && num_kb < forced)) continue;
+      for (int tokens : {16, 32, 48, 64}) consider(1, split, info.clusters[i], tokens);
     }
   }
   return plan;
@@ -891,42 +862,37 @@ static int32_t launch(const void* q, int64_t ldq, const int8_t* w, int64_t ldw, 
                       Params& p, int variant, cudaStream_t st) {
   const DeviceInfo* info = nullptr;
   if (int32_t rc = device_info(&info)) return rc;
-  const int64_t sms = sm_count();
-  int form = choose_form(p, sms);
-  if (variant == 2) form = kPair;
-  if (variant != 0 && variant != 2 && form == kPair) form = kSplit64;
-  const bool pair = form == kPair;
-  const int num_kb = static_cast<int>((p.K + BK - 1) / BK);
-  Plan plan = {256, 256, 2, sms / 2};
-  if (pair)
-    plan.tokens = pair_tokens(p, num_kb, sms / 2);
-  else
-    plan = split_plan(p, form == kSplit16 ? Cfg<kSplit16>::kTokens : Cfg<kSplit64>::kTokens, num_kb, *info,
-                      variant > 2 ? 1 << (variant - 3) : 0);
+  const Plan plan = make_plan(p, *info, sm_count(), variant);
+  const bool pair = plan.ctas == 2;
   p.tokens = plan.tokens;
   p.tile_rows = plan.tile_rows;
-  p.split = pair ? 1 : plan.cluster;
+  p.split = plan.split;
+  p.stage_bytes = A_BYTES + plan.tokens / plan.ctas * BK;
+  const int fit = (pair ? Cfg<2>::kRing : Cfg<1>::kRing) / p.stage_bytes;
+  p.stages = fit < MAX_STAGES ? fit : MAX_STAGES;
   CUtensorMap map_w, map_q, map_q_full;
   if (int32_t rc = encode_tensor_map_3d(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, p.K, p.N, p.E, ldw, group_stride, BK,
-                                        pair ? WROWS : plan.tile_rows, CU_TENSOR_MAP_SWIZZLE_128B))
+                                        plan.tile_rows / plan.ctas, CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
   if (int32_t rc = encode_tensor_map_2d(&map_q, CU_TENSOR_MAP_DATA_TYPE_UINT8, q, p.K, p.R, ldq, BK,
-                                        pair ? Cfg<kPair>::kBox : Cfg<kSplit64>::kBox, CU_TENSOR_MAP_SWIZZLE_128B))
+                                        pair ? Cfg<2>::kBox : Cfg<1>::kBox, CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
   if (int32_t rc = encode_tensor_map_2d(&map_q_full, CU_TENSOR_MAP_DATA_TYPE_UINT8, q, p.K, p.R, ldq, BK,
-                                        pair ? plan.tokens / 2 : plan.tokens, CU_TENSOR_MAP_SWIZZLE_128B))
+                                        plan.tokens / plan.ctas, CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
   // kind::i8: D s32 (2) in bits [4,6); A (weight, s8 = 1) in [7,10), B (codes, s8 = 1 or u8 = 0) in [10,13); both
   // K-major; N >> 3 in [17,23) is filled in per tile; M >> 4 in [24,29)
   p.idesc = (2u << 4) | (1u << 7) | ((q_unsigned ? 0u : 1u) << 10) |
-            (static_cast<uint32_t>((pair ? 256 : 128) >> 4) << 24);
+            (static_cast<uint32_t>((128 * plan.ctas) >> 4) << 24);
   const int64_t tiles = row_tiles(p, plan.tokens) * ((p.N + plan.tile_rows - 1) / plan.tile_rows);
   if (tiles > 0x7fffffffLL) return fail(LC_ERR_UNSUPPORTED, "grouped_linear: too many tiles");
   const int64_t units = plan.units < tiles ? plan.units : tiles;
+  const int cluster = plan.ctas * plan.split;
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attrs[2];
-  launch_config(&cfg, attrs, static_cast<unsigned>(units * plan.cluster), smem_of(form), plan.cluster, st);
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel_for(form, p.out_dtype, p.act), map_w, map_q, map_q_full, p);
+  launch_config(&cfg, attrs, static_cast<unsigned>(units * cluster), pair ? smem_bytes<2>() : smem_bytes<1>(), cluster, st);
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, pair ? kernel_for<2>(p.out_dtype, p.act) : kernel_for<1>(p.out_dtype, p.act),
+                                             map_w, map_q, map_q_full, p);
   if (err != cudaSuccess) return fail(LC_ERR_CUDA, "grouped_linear: %s", cudaGetErrorString(err));
   return check_launch("grouped_linear");
 }

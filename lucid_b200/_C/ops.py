@@ -429,7 +429,7 @@ def expert_linear(x2d, wq, sw, bias, positions, offsets, rows: int, activation: 
         groups, n, ldw, stride = shape[0], shape[1], strides[1], strides[0]
     else:
         groups, n, ldw, stride = 1, shape[0], strides[0], 0
-    out = torch.empty((rows, width), dtype=out_dtype, device=dev)
+    out = x2d.new_empty((rows, width)) if out_dtype is x2d.dtype else torch.empty((rows, width), dtype=out_dtype, device=dev)
     need = (rows * ((k + 15) & -16) + 255 & -256) + (rows * 4 + 255 & -256)  # lc_expert_linear_workspace_bytes
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     _call_on(dev, _expert_linear, x2d.data_ptr(), _DTYPE[x2d.dtype], x_rows, x2d.stride(0),
@@ -451,8 +451,8 @@ def route_experts(logits, top_k: int, renormalize: bool):
         logits = logits.contiguous()
     t, e = logits.shape
     weights = torch.empty((t, top_k), dtype=torch.float32, device=dev)
-    experts = torch.empty((t, top_k), dtype=torch.int32, device=dev)
-    positions = torch.empty((t, top_k), dtype=torch.int32, device=dev)
+    experts = torch.empty_like(weights, dtype=torch.int32)
+    positions = torch.empty_like(experts)
     offsets = torch.empty(e + 1, dtype=torch.int32, device=dev)
     ws, need = None, 0
     if t > _ROUTE_ONE_CTA:
@@ -468,7 +468,7 @@ def combine_experts(y, weights, positions, residual, dev: torch.device) -> torch
     """``sum_j weights[t, j] * y[positions[t, j]] (+ residual[t])`` (``lc_combine_experts``)."""
     t, top_k = positions.shape
     rows, cols = y.shape
-    out = torch.empty((t, cols), dtype=y.dtype, device=dev)
+    out = y.new_empty((t, cols)) if residual is None else torch.empty_like(residual, memory_format=torch.contiguous_format)
     _call_on(dev, _combine_experts, y.data_ptr(), _DTYPE[y.dtype], rows, cols, y.stride(0), weights.data_ptr(),
              positions.data_ptr(), t, top_k, None if residual is None else residual.data_ptr(),
              0 if residual is None else residual.stride(0), out.data_ptr(), cols)

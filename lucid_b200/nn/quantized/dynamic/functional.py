@@ -97,9 +97,10 @@ def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
     """``x`` as a matrix whose rows are dense (any row pitch)."""
     if x.dtype not in _FLOATS:
         raise TypeError(f"{what} must be float32, bfloat16 or float16, got {x.dtype}")
-    if x.dim() != 2:
-        x = x.reshape(-1, x.shape[-1])
     strides = x.stride()
+    if len(strides) != 2:
+        x = x.reshape(-1, x.shape[-1])
+        strides = x.stride()
     return x if strides[1] == 1 and strides[0] >= x.shape[1] else x.contiguous()
 
 
@@ -110,9 +111,9 @@ def _vector(t: torch.Tensor | None, shape: tuple, name: str, device: torch.devic
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
     if t.device != device:
         raise RuntimeError(f"tensors on different devices: {device} and {t.device}")
-    if t.dtype is not torch.float32:
-        t = t.float()
-    return t if t.is_contiguous() else t.contiguous()
+    if t.dtype is torch.float32 and t.is_contiguous():
+        return t
+    return t.float().contiguous()
 
 
 def _residual(t: torch.Tensor | None, shape: tuple, dtype: torch.dtype, device: torch.device):
