@@ -301,7 +301,7 @@ int32_t lc_dynamic_linear_f32(const float* x, int64_t ldx, int64_t M, int64_t K,
 /* ---- int8 Linear with a fused epilogue, one or many groups -------------
  * The dynamically quantized Linear (lucid/nn/quantized/dynamic/linear.py:85-92) with what a transformer
  * block puts behind it, and the same product grouped by expert (the reference has neither):
- *   out[m,n] = act(f32(acc - zx*wsum[e,n]) * sx[m] * sw[e,n] + bias[e,n]) + residual[m,n],
+ *   out[m,n] = act(f32(acc - zx*wsum[e,n]) * (sx[m] * sw[e,n]) + bias[e,n]) + residual[m,n],
  *   acc      = sum_k q[m,k] * wq[e,n,k]  (int32, exact),  e = the group whose rows contain m.
  * q [rows, ldq]: int8 (or uint8, q_unsigned) codes, rows sorted by group; offsets [groups + 1] on the device:
  * group e owns rows offsets[e] .. offsets[e+1] (ascending; values are clamped to [0, rows]).  offsets NULL:

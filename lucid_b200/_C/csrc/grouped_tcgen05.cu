@@ -1,7 +1,7 @@
 // int8 Linear of one or many groups with bias, activation and residual in its epilogue, for B200:
 //
 //   acc[m,n] = sum_k q[m,k] * w[e,n,k]                     e = group (expert) that owns row m
-//   out[m,n] = act(f32(acc - zx*wsum[e,n]) * sx[m] * sw[e,n] + bias[e,n]) + residual[m,n]
+//   out[m,n] = act(f32(acc - zx*wsum[e,n]) * (sx[m] * sw[e,n]) + bias[e,n]) + residual[m,n]
 //
 // The rows of q are sorted by group; offsets[e] .. offsets[e+1] are the rows of group e and live on the
 // device, so nothing of the routing is read on the host.  One group without offsets is the dense Linear.
@@ -41,9 +41,9 @@ constexpr int BK = 128;               // bytes of K per stage = one 128B swizzle
 constexpr int UMMA_K = 32;
 constexpr int WROWS = 128;            // weight rows a CTA loads per tile
 constexpr int A_BYTES = WROWS * BK;
-constexpr int NUM_THREADS = 320;
-constexpr int EPI_WARPS = 8;
+constexpr int EPI_WARPS = 8;          // two per TMEM lane quadrant (four: the same times, decode batches 4 % slower)
 constexpr int EPI_THREADS = EPI_WARPS * 32;
+constexpr int NUM_THREADS = 64 + EPI_THREADS;
 constexpr int MAX_GROUPS = 1024;
 
 // kTokens: most rows of q per tile; kStep: granularity of the instruction's N; kBox: rows of q per TMA box of a tile
@@ -218,10 +218,15 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// v * Phi(v), Phi the normal distribution function.  Phi(-a) = 2^p(a) for a = |v|, p a polynomial of degree 9 fitted
-// to log2 Phi(-a) on [0, 6] (least squares over Chebyshev nodes, reweighted towards the smallest largest error in
-// a * Phi): a * Phi(-a) is off by at most 3.5e-8, and by 2e-12 beyond 6.  15 instructions where the library's erff
-// takes about 40: on an 8192 x 2048 x 512 product, whose time is the epilogue's, 45 us against TODO us.
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// v * Phi(v) = max(v, 0) - a Phi(-a), a = |v|, Phi the normal distribution function.  Phi(-a) = 2^p(a), p a polynomial
+// of degree 9 fitted to log2 Phi(-a) on [0, 6] (least squares over Chebyshev nodes, reweighted towards the smallest
+// largest error in a * Phi): a * Phi(-a) is off by at most 3.5e-8, and by 2e-12 beyond 6.  13 instructions where the
+// library's erff takes about 40: an 8192 x 2048 x 512 product, whose time is the epilogue's, 45 us against TODO us.
 __device__ __forceinline__ float gelu(float v) {
   const float a = fminf(fabsf(v), 10.0f);
   float p = 2.9685912750210264e-07f;
@@ -234,8 +239,7 @@ __device__ __forceinline__ float gelu(float v) {
   p = fmaf(p, a, -0.4592026472091675f);
   p = fmaf(p, a, -1.151106357574463f);
   p = fmaf(p, a, -0.9999999403953552f);
-  const float t = exp2_approx(p);
-  return v * (v > 0.0f ? 1.0f - t : t);
+  return fmaf(-a, exp2_approx(p), max_nan(v, 0.0f));
 }
 
 template <int ACT>
@@ -292,7 +296,7 @@ __device__ __forceinline__ void drain(const Params& p, const Lane& l) {
   const int64_t row0 = l.m0 + (ACT == LC_ACT_SWIGLU ? up : 0);
   const T* const res = static_cast<const T*>(p.residual);
 #pragma unroll 1
-  for (int c = l.first; c < l.rows; c += 2 * CH) {
+  for (int c = l.first; c < l.rows; c += EPI_WARPS / 4 * CH) {
     const int left = l.in ? l.rows - c : 0;
     constexpr int kStep = ACT == LC_ACT_SWIGLU ? 2 : 1;  // a lane finishes every row, or every second one
     T rv[CH / kStep];
@@ -317,18 +321,20 @@ __device__ __forceinline__ void drain(const Params& p, const Lane& l) {
         }
       }
     }
+    if (p.zx) {
+#pragma unroll
+      for (int j = 0; j < CH; ++j) r[j] -= static_cast<uint32_t>(l.corr);
+    }
     float f[CH];
 #pragma unroll
     for (int j = 0; j < CH; j += 4) {
       const float4 s = *reinterpret_cast<const float4*>(l.sx + c + j);
       const float sv[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        f[j + i] = __fadd_rn(__fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(r[j + i]) - l.corr), sv[i]), l.sw), l.bias);
+      for (int i = 0; i < 4; ++i) f[j + i] = fmaf(static_cast<float>(static_cast<int>(r[j + i])), sv[i] * l.sw, l.bias);
     }
-    T* o = static_cast<T*>(p.out) + (row0 + c) * p.ldo + col;
-#pragma unroll
-    for (int j = 0; j < CH; j += kStep) {
+    T* const o = static_cast<T*>(p.out) + (row0 + c) * p.ldo + col;
+    auto finish = [&](int j) {  // the result of row c + j
       float v;
       if constexpr (ACT == LC_ACT_SWIGLU) {
         // lanes 8 apart hold the gate and the up value of one unit: each finishes every other row
@@ -338,11 +344,18 @@ __device__ __forceinline__ void drain(const Params& p, const Lane& l) {
       } else {
         v = activate<ACT>(f[j]);
       }
-      if (j + (kStep == 2 ? up : 0) < left) {
-        if (res) v += widen<T>(rv[j / kStep]);
-        *o = narrow<T>(v);
+      if (res) v += widen<T>(rv[j / kStep]);
+      return narrow<T>(v);
+    };
+    if (__all_sync(0xffffffffu, left >= CH)) {
+#pragma unroll
+      for (int j = 0; j < CH; j += kStep) o[j * p.ldo] = finish(j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < CH; j += kStep) {
+        const T v = finish(j);
+        if (j + (kStep == 2 ? up : 0) < left) o[j * p.ldo] = v;
       }
-      o += kStep * p.ldo;
     }
   }
 }
@@ -373,7 +386,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   const uint32_t part_bar = bar_base + 8u * (2 * MAX_STAGES + 4);  // rank 0: the other ranks' sums have been added
   const uint32_t free_bar = part_bar + 8u;                     // other ranks: rank 0's buffer is zero again
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (known to be uniform)
   const long long budget = p.wait_test ? 20000LL : kWaitCycles;
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
@@ -620,19 +633,36 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     if (p.early_weights) pdl_wait();
     const int zx = p.zx ? __float2int_rn(__ldg(p.zx)) : 0;
     TileWalk walk(s_start, s_off, tiles_n, p);
+    const int cta_rows = p.tile_rows / CG, local = q * 32 + lane;  // this lane's weight row among the CTA's
+    // a tile's scales and biases, fetched while the tile before it is drained
+    struct Side {
+      Tile tile;
+      int64_t n;
+      bool in;
+      float sx, sw, bias;
+      int corr;
+    };
+    auto fetch = [&](int t) {
+      Side s;
+      s.tile = walk.at(t);
+      s.n = s.tile.n0 + (CG == 2 ? static_cast<int64_t>(rank) * cta_rows : 0) + local;
+      s.in = s.n < p.N && local < cta_rows;  // lanes beyond a narrow tile hold nothing
+      const int64_t at = static_cast<int64_t>(s.tile.e) * p.N + s.n;
+      s.sx = et < s.tile.rows ? __ldg(p.sx + (p.sx_per_row ? s.tile.m0 + et : 0)) : 0.0f;
+      s.sw = s.in ? __ldg(p.sw + at) : 0.0f;
+      s.bias = (s.in && p.bias) ? __ldg(p.bias + at) : 0.0f;
+      s.corr = (s.in && p.wsum) ? zx * __ldg(p.wsum + at) : 0;
+      return s;
+    };
+    Side next = {};
+    if (unit < total) next = fetch(unit);
     int it = 0;
     for (int t = unit; t < total; t += units, ++it) {
-      const Tile tile = walk.at(t);
+      const Side side = next;
+      const Tile& tile = side.tile;
       const int as = it & 1;
       float* const sx = s_sx + as * C::kTokens;
-      if (et < C::kTokens) sx[et] = et < tile.rows ? __ldg(p.sx + (p.sx_per_row ? tile.m0 + et : 0)) : 0.0f;
-      const int cta_rows = p.tile_rows / CG;
-      const int64_t n = tile.n0 + (CG == 2 ? static_cast<int64_t>(rank) * cta_rows : 0) + q * 32 + lane;
-      const int64_t at = static_cast<int64_t>(tile.e) * p.N + n;
-      const bool in = n < p.N && q * 32 + lane < cta_rows;  // lanes beyond a narrow tile hold nothing
-      const float sw = in ? __ldg(p.sw + at) : 0.0f;
-      const float bias = (in && p.bias) ? __ldg(p.bias + at) : 0.0f;
-      const int corr = (in && p.wsum) ? zx * __ldg(p.wsum + at) : 0;
+      if (et < C::kTokens) sx[et] = side.sx;
       if (CG == 1 && p.split > 1 && leader && et == 0)
         mbar_expect_tx(part_bar, static_cast<uint32_t>((p.split - 1) * tile.rows * WROWS * 4));
       bool arrived = mbar_wait(acc_full_bar(as), (it >> 1) & 1, budget);
@@ -647,24 +677,25 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         break;
       }
       tc_fence_after();
+      if (t + units < total) next = fetch(t + units);
       Lane l;
       l.t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(as * C::kTokens);
       l.m0 = tile.m0;
       l.rows = tile.rows;
-      l.n = n;
-      l.in = in;
-      l.sw = sw;
-      l.bias = bias;
-      l.corr = corr;
+      l.n = side.n;
+      l.in = side.in;
+      l.sw = side.sw;
+      l.bias = side.bias;
+      l.corr = side.corr;
       l.sx = sx;
       l.first = group * CH;
-      l.slot = q * 32 + lane;
+      l.slot = local;
       l.red = CG == 1 && p.split > 1 ? s_red : nullptr;
       if (CG == 1 && !leader) {
         const uint32_t dst = map_to_cta(red_base, 0) + static_cast<uint32_t>(l.slot) * 4;
         const uint32_t bar = map_to_cta(part_bar, 0);
 #pragma unroll 1
-        for (int c = l.first; c < l.rows; c += 2 * CH) {
+        for (int c = l.first; c < l.rows; c += EPI_WARPS / 4 * CH) {
           uint32_t r[CH];
           tc_ld(l.t_row + static_cast<uint32_t>(c), r);
           tc_wait_ld();
