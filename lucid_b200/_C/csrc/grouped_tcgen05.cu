@@ -386,7 +386,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   const uint32_t part_bar = bar_base + 8u * (2 * MAX_STAGES + 4);  // rank 0: the other ranks' sums have been added
   const uint32_t free_bar = part_bar + 8u;                     // other ranks: rank 0's buffer is zero again
 
-  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (known to be uniform)
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long budget = p.wait_test ? 20000LL : kWaitCycles;
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
@@ -499,7 +499,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     // The whole warp walks the loop and one elected lane issues: in code that only lane 0 reaches, every operand of
     // a copy or an MMA is moved to a uniform register first, 70 clocks an instruction.
     int stage = 0;
-    uint32_t phase = 0;
+    uint32_t phase = 0, slot = tiles_base;
     bool ok = true;
     if (p.early_weights) pdl_wait();  // the codes are the previous kernel's
     TileWalk walk(s_start, s_off, tiles_n, p);
@@ -513,8 +513,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       const int n0 = static_cast<int>(tile.n0) + (CG == 2 ? static_cast<int>(rank) * (p.tile_rows / 2) : 0);
       const int m0 = tile.m0 + (CG == 2 ? static_cast<int>(rank) * mine : 0);
       const int e = tile.e;
-      auto load_q = [&](int s, int kb) {
-        const uint32_t dst = tiles_base + s * stage_bytes + A_BYTES;
+      auto load_q = [&](int s, uint32_t dst, int kb) {
         if (full) {
           if constexpr (CG == 2)
             tma_load_2d_pair(dst, &tmap_q_full, kb * BK, m0, map_to_cta(full_bar(s), 0));
@@ -532,11 +531,12 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       int kb = kb0;
       if (CG == 1 && t == unit && ahead) {  // the first stages have their weights under way
         if (elect_one())
-          for (int s = 0; s < ahead; ++s) load_q(s, kb0 + s);
+          for (int s = 0; s < ahead; ++s) load_q(s, tiles_base + s * stage_bytes + A_BYTES, kb0 + s);
         __syncwarp();
         kb = kb0 + ahead;
         stage = ahead % stages;
         phase = ahead == stages ? 1u : 0u;
+        slot = tiles_base + stage * stage_bytes;
       }
       for (; kb < kb1; ++kb) {
         if (!__all_sync(0xffffffffu, mbar_wait(empty_bar(stage), phase ^ 1u, budget))) {
@@ -545,22 +545,23 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
           break;
         }
         if (elect_one()) {
-          const uint32_t dst = tiles_base + stage * stage_bytes;
           if (CG == 1 || leader) mbar_expect_tx(full_bar(stage), bytes);
           if constexpr (CG == 2)
-            tma_load_3d_pair(dst, &tmap_w, kb * BK, n0, e, map_to_cta(full_bar(stage), 0));
+            tma_load_3d_pair(slot, &tmap_w, kb * BK, n0, e, map_to_cta(full_bar(stage), 0));
           else
-            tma_load_3d(dst, &tmap_w, kb * BK, n0, e, full_bar(stage));
-          load_q(stage, kb);
+            tma_load_3d(slot, &tmap_w, kb * BK, n0, e, full_bar(stage));
+          load_q(stage, slot + A_BYTES, kb);
         }
         __syncwarp();
         if (CG == 1 || leader) {
           armed |= 1u << stage;
           armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
         }
+        slot += stage_bytes;
         if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
+          slot = tiles_base;
         }
       }
     }
@@ -574,6 +575,9 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       int stage = 0, it = 0;
       uint32_t phase = 0;
       bool ok = true;
+      // descriptors of the first stage; a stage further on is stage_bytes / 16 more (the start address is below 2^18)
+      const uint64_t w_first = make_smem_desc(tiles_base), q_off = A_BYTES >> 4;
+      uint64_t w_desc = w_first;
       TileWalk walk(s_start, s_off, tiles_n, p);
       for (int t = unit; t < total && ok; t += units, ++it) {
         const Tile tile = walk.at(t);
@@ -594,8 +598,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
           }
           tc_fence_after();
           if (elect_one()) {
-            const uint32_t src = tiles_base + stage * stage_bytes;
-            const uint64_t w_desc = make_smem_desc(src), q_desc = make_smem_desc(src + A_BYTES);
+            const uint64_t q_desc = w_desc + q_off;
 #pragma unroll
             for (int j = 0; j < BK / UMMA_K; ++j) {
               const uint64_t koff = static_cast<uint64_t>((j * UMMA_K) >> 4);
@@ -611,9 +614,11 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
               tc_commit(empty_bar(stage));
           }
           __syncwarp();
+          w_desc += static_cast<uint32_t>(stage_bytes) >> 4;
           if (++stage == stages) {
             stage = 0;
             phase ^= 1u;
+            w_desc = w_first;
           }
         }
         if (ok && elect_one()) {
@@ -856,34 +861,45 @@ static Plan make_plan(const Params& p, const DeviceInfo& info, int64_t sms, int 
     groups = static_cast<double>(p.E) * (1.0 - empty);
   }
   const double rows = static_cast<double>(p.R) / groups;
-  const int step = p.act == LC_ACT_SWIGLU ? 16 : 8;  // gate and up rows of a unit stay in one tile
+  const int64_t step = p.act == LC_ACT_SWIGLU ? 16 : 8;  // gate and up rows of a unit stay in one tile
   Plan plan = {2, 256, 256, 1, sms / 2};
   double best = 0.0;
   auto consider = [&](int ctas, int split, int64_t units, int tokens) {
     const double row_tiles = groups * ceil(rows / tokens), cols = rows < tokens ? rows : tokens;
-    for (int cta_rows = 128; cta_rows >= 48; cta_rows -= step) {
-      const double tiles = row_tiles * static_cast<double>((p.N + ctas * cta_rows - 1) / (ctas * cta_rows));
-      const double waves = p.offsets ? tiles / units + 0.5 : ceil(tiles / units);
-      // (weights that only one row tile reads come from HBM, of which a CTA gets less than of the L2)
-      const double load = cta_rows * BK / (rows <= tokens ? 40.0 : 64.0) + cols / ctas * BK / 64.0;
-      double block = ctas * cols > 300.0 ? ctas * cols : 300.0;
-      if (load > block) block = load;
-      const double loop = (num_kb + split - 1) / split * block, drain = 25.0 * cols;
-      const double cost = waves * ((loop > drain ? loop : drain) + (split > 1 ? 2100.0 : 600.0)) + (loop > drain ? drain : loop);
-      if (best == 0.0 || cost < 0.98 * best) {
-        best = cost;
-        plan = {ctas, tokens, ctas * cta_rows, split, units};
-      }
+    int64_t cta_rows = 128, across = (p.N + ctas * 128 - 1) / (ctas * 128);
+    double waves = row_tiles * static_cast<double>(across) / static_cast<double>(units);
+    if (p.offsets) {
+      waves += 0.5;
+    } else {
+      waves = ceil(waves);
+    }
+    if (!p.offsets && rows <= tokens) {  // weights read once: as few rows as the same number of waves allows
+      const int64_t room = static_cast<int64_t>(waves * static_cast<double>(units) / row_tiles);
+      cta_rows = ((p.N + room * ctas - 1) / (room * ctas) + step - 1) / step * step;
+      if (cta_rows < 48) cta_rows = 48;
+      if (cta_rows > 128) cta_rows = 128;
+    }
+    // (weights that only one row tile reads come from HBM, of which a CTA gets less than of the L2)
+    const double load = static_cast<double>(cta_rows * BK) / (rows <= tokens ? 40.0 : 64.0) + cols / ctas * BK / 64.0;
+    double block = ctas * cols > 300.0 ? ctas * cols : 300.0;
+    if (load > block) block = load;
+    const double loop = (num_kb + split - 1) / split * block, drain = 25.0 * cols;
+    const double cost = waves * ((loop > drain ? loop : drain) + (split > 1 ? 2100.0 : 600.0)) + (loop > drain ? drain : loop);
+    if (best == 0.0 || cost < 0.98 * best) {
+      best = cost;
+      plan = {ctas, tokens, static_cast<int>(ctas * cta_rows), split, units};
     }
   };
   if (variant == 0 || variant == 2)
     for (int tokens : {64, 128, 192, 256}) consider(2, 1, sms / 2, tokens);
   if (variant != 2) {
+    const double most = p.offsets ? 2.0 * rows : rows;  // groups differ in size
+    const int tokens = most > 48.0 ? 64 : (static_cast<int>(most) + 15) / 16 * 16;
     for (int i = 0; i < 4; ++i) {
       const int split = 1 << i;
       if (info.clusters[i] < 1 || num_kb < (forced ? 1 : 4) * split) break;
       if (forced && split != forced && !(i == 0 && num_kb < forced)) continue;
-      for (int tokens : {16, 32, 48, 64}) consider(1, split, info.clusters[i], tokens);
+      consider(1, split, info.clusters[i], tokens < 16 ? 16 : tokens);
     }
   }
   return plan;

@@ -24,6 +24,7 @@ from lucid_b200 import _backend
 
 ACTIVATIONS = (None, "relu", "gelu", "gelu_tanh", "silu", "swiglu")
 _ACTIVATION_ID = {name: i for i, name in enumerate(ACTIVATIONS)}
+_SWIGLU = _ACTIVATION_ID["swiglu"]
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 
@@ -104,9 +105,7 @@ def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
     return x if strides[1] == 1 and strides[0] >= x.shape[1] else x.contiguous()
 
 
-def _vector(t: torch.Tensor | None, shape: tuple, name: str, device: torch.device):
-    if t is None:
-        return None
+def _vector(t: torch.Tensor, shape: tuple, name: str, device: torch.device) -> torch.Tensor:
     if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
     if t.device != device:
@@ -116,9 +115,7 @@ def _vector(t: torch.Tensor | None, shape: tuple, name: str, device: torch.devic
     return t.float().contiguous()
 
 
-def _residual(t: torch.Tensor | None, shape: tuple, dtype: torch.dtype, device: torch.device):
-    if t is None:
-        return None
+def _residual(t: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
     if t.shape != shape:
         raise ValueError(f"residual has shape {tuple(t.shape)}, expected {shape}")
     if t.dtype is not dtype:
@@ -132,7 +129,7 @@ def _activation(name, n: int) -> int:
     code = _ACTIVATION_ID.get(name)
     if code is None:
         raise ValueError(f"activation must be one of {ACTIVATIONS}, got {name!r}")
-    if name == "swiglu" and n % 16:
+    if code == _SWIGLU and n % 16:
         raise ValueError("swiglu needs weight rows in interleaved blocks of 8 gate and 8 up rows "
                          f"(a multiple of 16), got {n}")
     return code
@@ -142,13 +139,18 @@ def _check_cuda(x: torch.Tensor, device: torch.device) -> None:
     if not x.is_cuda:
         raise RuntimeError("the quantized kernels take CUDA tensors only (there is no CPU fallback); "
                            f"got a tensor on {x.device}")
-    if device != x.device:
+    if x.device != device:
         raise RuntimeError(f"tensors on different devices: {x.device} and {device}")
 
 
-def _result_type(x: torch.Tensor, out_dtype) -> torch.dtype:
-    if out_dtype is None:
-        return x.dtype
+def _matrix(weight: torch.Tensor) -> tuple:
+    shape = weight.shape
+    if len(shape) != 2:
+        raise ValueError(f"weight must be [N, K], got {tuple(shape)}")
+    return shape
+
+
+def _result_type(out_dtype) -> torch.dtype:
     if out_dtype not in _FLOATS:
         raise TypeError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
     return out_dtype
@@ -165,27 +167,27 @@ def linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bi
     rows; the result has N / 2 columns).  ``residual`` has the result's shape and is added after the
     activation.  The result has ``out_dtype`` (default: the type of ``x``), which ``residual`` must
     have too."""
-    if weight.dim() != 2:
-        raise ValueError(f"weight must be [N, K], got {tuple(weight.shape)}")
-    n, k = weight.shape
-    if x.dim() < 1 or x.shape[-1] != k:
-        raise ValueError(f"input of shape {tuple(x.shape)} does not contract with a [{n}, {k}] weight")
+    n, k = _matrix(weight)
+    shape = x.shape
+    if not shape or shape[-1] != k:
+        raise ValueError(f"input of shape {tuple(shape)} does not contract with a [{n}, {k}] weight")
     device = x.device
     _check_cuda(x, weight.device)
     x2 = _rows(x, "input")
     act = _activation(activation, n)
-    dtype = _result_type(x, out_dtype)
-    width = n // 2 if activation == "swiglu" else n
-    shape = (*x.shape[:-1], width)
-    residual = _residual(residual, shape, dtype, device)
-    scale = _vector(weight_scale, (n,), "weight_scale", device)
-    bias = _vector(bias, (n,), "bias", device)
+    dtype = x.dtype if out_dtype is None else _result_type(out_dtype)
+    width = n // 2 if act == _SWIGLU else n
     rows = x2.shape[0]
+    if residual is not None:
+        residual = _residual(residual, (rows, width) if x2 is x else (*shape[:-1], width), dtype, device)
+    scale = _vector(weight_scale, (n,), "weight_scale", device)
+    if bias is not None:
+        bias = _vector(bias, (n,), "bias", device)
     if rows == 0 or n == 0:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return torch.empty((*shape[:-1], width), dtype=dtype, device=device)
     y = _backend.ops().expert_linear(x2, pack_weight(weight), scale, bias, None, None, rows, act, residual, width, dtype,
                                      device)
-    return y if x2 is x else y.view(shape)
+    return y if x2 is x else y.view((*shape[:-1], width))
 
 
 def route_experts(logits: torch.Tensor, top_k: int, *, renormalize: bool = True) -> ExpertRouting:
@@ -238,10 +240,11 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Ten
     _check_cuda(x, routing.positions.device)
     x2 = _rows(x, "input")
     act = _activation(activation, n)
-    dtype = _result_type(x, out_dtype)
-    width = n // 2 if activation == "swiglu" else n
+    dtype = x.dtype if out_dtype is None else _result_type(out_dtype)
+    width = n // 2 if act == _SWIGLU else n
     scale = _vector(weight_scale, (e, n), "weight_scale", device)
-    bias = _vector(bias, (e, n), "bias", device)
+    if bias is not None:
+        bias = _vector(bias, (e, n), "bias", device)
     if rows == 0 or n == 0:
         return torch.empty((rows, width), dtype=dtype, device=device)
     return _backend.ops().expert_linear(x2, pack_weight(weight), scale, bias, None if sorted_rows else routing.positions,
@@ -258,7 +261,8 @@ def combine_experts(y: torch.Tensor, routing: ExpertRouting, *, residual: torch.
     _check_cuda(y, routing.positions.device)
     y = _rows(y, "y")
     shape = (routing.tokens, y.shape[1])
-    residual = _residual(residual, shape, y.dtype, device)
+    if residual is not None:
+        residual = _residual(residual, shape, y.dtype, device)
     if shape[0] == 0 or shape[1] == 0:
         return torch.empty(shape, dtype=y.dtype, device=device)
     return _backend.ops().combine_experts(y, routing.weights, routing.positions, residual, device)
