@@ -333,7 +333,7 @@ __device__ __forceinline__ void drain(const Params& p, const Lane& l) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) f[j + i] = fmaf(static_cast<float>(static_cast<int>(r[j + i])), sv[i] * l.sw, l.bias);
     }
-    T* const o = static_cast<T*>(p.out) + (row0 + c) * p.ldo + col;
+    T* o = static_cast<T*>(p.out) + (row0 + c) * p.ldo + col;
     auto finish = [&](int j) {  // the result of row c + j
       float v;
       if constexpr (ACT == LC_ACT_SWIGLU) {
@@ -349,12 +349,12 @@ __device__ __forceinline__ void drain(const Params& p, const Lane& l) {
     };
     if (__all_sync(0xffffffffu, left >= CH)) {
 #pragma unroll
-      for (int j = 0; j < CH; j += kStep) o[j * p.ldo] = finish(j);
+      for (int j = 0; j < CH; j += kStep, o += kStep * p.ldo) *o = finish(j);
     } else {
 #pragma unroll
-      for (int j = 0; j < CH; j += kStep) {
+      for (int j = 0; j < CH; j += kStep, o += kStep * p.ldo) {
         const T v = finish(j);
-        if (j + (kStep == 2 ? up : 0) < left) o[j * p.ldo] = v;
+        if (j + (kStep == 2 ? up : 0) < left) *o = v;
       }
     }
   }
