@@ -388,7 +388,11 @@ def grouped_qlinear_i8(q, wq, sx, sw, bias=None, offsets=None, zx=None, wsum=Non
     rows = q.shape[0]
     width = n // 2 if activation == "swiglu" else n
     out = torch.empty((rows, width), dtype=out_dtype, device=dev)
-    sx = _f32c(sx).reshape(-1)
+    sx, sw = _f32c(sx).reshape(-1), _f32c(sw)
+    bias = None if bias is None else _f32c(bias)
+    zx = None if zx is None else _f32c(zx).reshape(-1)
+    if sw.numel() != groups * n or (bias is not None and bias.numel() != groups * n):
+        raise ValueError(f"grouped_qlinear_i8: sw and bias must have {groups * n} entries")
     if sx.numel() not in (1, rows):
         raise ValueError(f"grouped_qlinear_i8: sx has {sx.numel()} entries, expected 1 or {rows}")
     with _on(dev):

@@ -13,6 +13,10 @@ selects the activation grid: ``"tensor_affine"`` (reference default),
 ``"tensor_symmetric"`` or ``"token_symmetric"`` (one scale per row of ``x``).
 Range, qparams and codes of the activations stay on the device: the forward contains
 no host synchronisation.
+
+``set_activation("gelu")`` (or ``"relu"``, ``"gelu_tanh"``, ``"silu"``) and ``forward(x, residual=r)``
+put what a transformer block does next into the product's epilogue:
+``act(x @ W^T + b) + r``, computed in fp32 and rounded once to the output type.
 """
 from __future__ import annotations
 
@@ -29,6 +33,7 @@ from lucid_b200.quantization._functional import quantize
 from lucid_b200.quantization._qscheme import QDtype, per_channel_symmetric, qint8, quint8
 
 _ACT_SCHEMES = ("tensor_affine", "tensor_symmetric", "token_symmetric")
+_EPILOGUES = (None, "relu", "gelu", "gelu_tanh", "silu")
 
 
 class _SharedInputCodes:
@@ -99,6 +104,7 @@ class Linear(nn.Module):
         self.act_qdtype: QDtype = quint8
         self.act_scheme = "tensor_affine"
         self.out_dtype = torch.float32
+        self.activation: str | None = None
         self.register_buffer("weight_int8", torch.zeros((out_features, in_features), dtype=torch.int8))
         self.register_buffer("weight_scale", torch.ones(out_features))
         self.register_buffer("weight_zero_point", torch.zeros(out_features))
@@ -115,6 +121,13 @@ class Linear(nn.Module):
             raise ValueError(f"act_scheme must be one of {_ACT_SCHEMES}, got {scheme!r}")
         self.act_scheme = scheme
         self.act_qdtype = qdtype if qdtype is not None else (quint8 if scheme == "tensor_affine" else qint8)
+        return self
+
+    def set_activation(self, activation: str | None) -> "Linear":
+        """Function applied to the product and its bias in the same kernel (before a residual)."""
+        if activation not in _EPILOGUES:
+            raise ValueError(f"activation must be one of {_EPILOGUES}, got {activation!r}")
+        self.activation = activation
         return self
 
     def _quantize_activations(self, x2: torch.Tensor):
@@ -141,7 +154,49 @@ class Linear(nn.Module):
         self._scratches[key] = (rows, buf)
         return buf, True
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def _shared_codes(self, x: torch.Tensor, x2: torch.Tensor, device: torch.device):
+        """Codes of ``x2``, taken from (or left for) a sibling layer inside :func:`share_quantized_input`."""
+        if not (x.is_cuda and _shared_input.active):
+            return self._quantize_activations(x2)
+        key = (self.act_scheme, self.act_qdtype.name, self.in_features, _backend.ops().capture_id(device),
+               torch.cuda.current_stream(device).cuda_stream)
+        hit = _shared_input.get(x, key)
+        if hit is None:
+            hit = self._quantize_activations(x2)
+            _shared_input.put(x, key, hit)
+        return hit
+
+    def _fused_forward(self, x: torch.Tensor, residual: torch.Tensor | None) -> torch.Tensor:
+        """Forward with an activation or a residual in the epilogue."""
+        ops = _backend.ops()
+        if self.weight_zero_point.is_cuda and x.is_cuda and x.device != self.weight_int8.device:
+            raise RuntimeError(f"input on {x.device} but weights on {self.weight_int8.device}")
+        xd = _backend.on_cuda(x)
+        shape = (*x.shape[:-1], self.out_features)
+        if residual is not None:
+            if tuple(residual.shape) != shape:
+                raise ValueError(f"residual has shape {tuple(residual.shape)}, expected {shape}")
+            if residual.is_cuda and residual.device != xd.device:
+                raise RuntimeError(f"input on {xd.device} but residual on {residual.device}")
+            residual = residual.to(device=xd.device, dtype=self.out_dtype).reshape(-1, self.out_features)
+            if residual.stride(1) != 1 or residual.stride(0) < self.out_features:
+                residual = residual.contiguous()
+        x2 = xd.reshape(-1, self.in_features)
+        if x2.shape[0] == 0:
+            y = torch.zeros((0, self.out_features), dtype=self.out_dtype, device=xd.device)
+        else:
+            wq, wsum = self._cache.get(_backend.on_cuda(self.weight_int8), self.weight_zero_point)
+            xq, sx, zx = self._shared_codes(x, x2 if x2.dtype is torch.float32 else x2.float(), xd.device)
+            y = ops.grouped_qlinear_i8(xq, wq, sx, _backend.on_cuda(self.weight_scale),
+                                       bias=None if self.bias is None else _backend.on_cuda(self.bias), zx=zx,
+                                       wsum=wsum if zx is not None else None, activation=self.activation,
+                                       residual=residual, out_dtype=self.out_dtype)
+        y = y.reshape(shape)
+        return y if x.is_cuda else y.to(x.device)
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        if self.activation is not None or residual is not None:
+            return self._fused_forward(x, residual)
         ops = _backend.ops()
         if (x.is_cuda and x.dtype is torch.float32 and not _shared_input.active and x.is_contiguous()
                 and self.weight_int8.device == x.device and x.numel() > 0 and hasattr(ops, "raw_stream")
@@ -165,17 +220,7 @@ class Linear(nn.Module):
         if x2.shape[0] == 0:
             y = torch.zeros((0, self.out_features), dtype=self.out_dtype, device=xd.device)
         else:
-            hit = None
-            if x.is_cuda and _shared_input.active:
-                key = (self.act_scheme, self.act_qdtype.name, self.in_features, ops.capture_id(xd.device),
-                       torch.cuda.current_stream(xd.device).cuda_stream)
-                hit = _shared_input.get(x, key)
-                if hit is None:
-                    hit = self._quantize_activations(x2)
-                    _shared_input.put(x, key, hit)
-            if hit is None:
-                hit = self._quantize_activations(x2)
-            xq, sx, zx = hit
+            xq, sx, zx = self._shared_codes(x, x2, xd.device)
             y = ops.qlinear_i8(xq, wq, sx, _backend.on_cuda(self.weight_scale),
                                bias=None if self.bias is None else _backend.on_cuda(self.bias), zx=zx,
                                wsum=wsum if zx is not None else None, out_dtype=self.out_dtype)
@@ -199,4 +244,5 @@ class Linear(nn.Module):
         return qmod
 
     def extra_repr(self) -> str:
-        return f"in_features={self.in_features}, out_features={self.out_features}, dynamic=True"
+        act = "" if self.activation is None else f", activation={self.activation}"
+        return f"in_features={self.in_features}, out_features={self.out_features}, dynamic=True{act}"
