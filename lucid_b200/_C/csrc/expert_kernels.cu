@@ -407,19 +407,23 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) quantize_tokens_kernel(
   pdl_launch_dependents();
   const int sub = threadIdx.x % TPR, warp = threadIdx.x >> 5;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / TPR;
-  const bool live = row < p.rows && (!p.valid || row < __ldg(p.valid));
+  const bool there = row < p.rows;
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
-  const int vectors = static_cast<int>(p.cols / VN);
+  const int vectors = static_cast<int>(p.cols / VN), copies = p.positions ? p.copies : 1;
   Vec16<T> v[ITEMS];
   float largest = 0.0f;
+  // the row, where it goes and whether it counts are requested together
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
     const int at = i * TPR + sub;
-    if (live && at < vectors) v[i].load(x + static_cast<int64_t>(at) * VN);
+    if (there && at < vectors) v[i].load(x + static_cast<int64_t>(at) * VN);
   }
+  int64_t to = row;
+  if (there && p.positions) to = __ldg(p.positions + row * copies);
+  const bool live = there && (!p.valid || row < __ldg(p.valid));
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
-    if (live && i * TPR + sub < vectors) largest = fmaxf(largest, largest_of(v[i]));
+    if (there && i * TPR + sub < vectors) largest = fmaxf(largest, largest_of(v[i]));
   }
   largest = warp_max(largest);
   if (TPR > 32) {
@@ -432,7 +436,6 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) quantize_tokens_kernel(
   }
   if (!live) return;
   const float s = token_scale(largest), inv = __fdiv_rn(1.0f, s);
-  const int copies = p.positions ? p.copies : 1;
   uint32_t packed[ITEMS][VN / 4];
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
@@ -443,10 +446,11 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) quantize_tokens_kernel(
                                           __fmul_rn(to_float<T>(v[i].v[j + 3]), inv), 0.0f, false);
   }
   for (int c = 0; c < copies; ++c) {
-    const int64_t to = p.positions ? __ldg(p.positions + row * copies + c) : row;
-    if (to < 0 || to >= p.out_rows) continue;
-    if (sub == 0) p.scale[to] = s;
-    int8_t* q = p.codes + to * p.ldq;
+    const int64_t row_out = to;
+    if (c + 1 < copies) to = __ldg(p.positions + row * copies + c + 1);
+    if (row_out < 0 || row_out >= p.out_rows) continue;
+    if (sub == 0) p.scale[row_out] = s;
+    int8_t* q = p.codes + row_out * p.ldq;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       const int at = i * TPR + sub;
@@ -455,6 +459,63 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) quantize_tokens_kernel(
           *reinterpret_cast<uint2*>(q + static_cast<int64_t>(at) * VN) = make_uint2(packed[i][0], packed[i][VN / 4 - 1]);
         else
           *reinterpret_cast<uint32_t*>(q + static_cast<int64_t>(at) * VN) = packed[i][0];
+      }
+    }
+  }
+}
+
+// rows too long for that: 256 threads read the row twice, the second time from the L2 (six rows a SM are 50 MB)
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_tokens_long_kernel(const TokenParams p) {
+  constexpr int VN = Vec16<T>::kN, UNROLL = 4;
+  __shared__ float s_max[8];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t row = blockIdx.x;
+  if (p.valid && row >= __ldg(p.valid)) return;
+  const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+  const int vectors = static_cast<int>(p.cols / VN);
+  float largest = 0.0f;
+  for (int i = threadIdx.x; i < vectors; i += UNROLL * 256) {
+    Vec16<T> v[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (i + u * 256 < vectors) v[u].load(x + static_cast<int64_t>(i + u * 256) * VN);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (i + u * 256 < vectors) largest = fmaxf(largest, largest_of(v[u]));
+  }
+  largest = warp_max(largest);
+  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = largest;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) largest = fmaxf(largest, s_max[w]);
+  const float s = token_scale(largest), inv = __fdiv_rn(1.0f, s);
+  const int copies = p.positions ? p.copies : 1;
+  for (int c = 0; c < copies; ++c) {
+    const int64_t to = p.positions ? __ldg(p.positions + row * copies + c) : row;
+    if (to < 0 || to >= p.out_rows) continue;
+    if (threadIdx.x == 0) p.scale[to] = s;
+    int8_t* q = p.codes + to * p.ldq;
+    for (int i = threadIdx.x; i < vectors; i += UNROLL * 256) {
+      Vec16<T> v[UNROLL];
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u)
+        if (i + u * 256 < vectors) v[u].load(x + static_cast<int64_t>(i + u * 256) * VN);
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        if (i + u * 256 >= vectors) continue;
+        uint32_t packed[VN / 4];
+#pragma unroll
+        for (int j = 0; j < VN; j += 4)
+          packed[j / 4] = pack4_sat<false>(__fmul_rn(to_float<T>(v[u].v[j]), inv), __fmul_rn(to_float<T>(v[u].v[j + 1]), inv),
+                                           __fmul_rn(to_float<T>(v[u].v[j + 2]), inv),
+                                           __fmul_rn(to_float<T>(v[u].v[j + 3]), inv), 0.0f, false);
+        int8_t* dst = q + static_cast<int64_t>(i + u * 256) * VN;
+        if (VN == 8)
+          *reinterpret_cast<uint2*>(dst) = make_uint2(packed[0], packed[VN / 4 - 1]);
+        else
+          *reinterpret_cast<uint32_t*>(dst) = packed[0];
       }
     }
   }
@@ -494,14 +555,14 @@ cudaError_t launch_tokens(const TokenParams& p, cudaStream_t st) {
   const bool vec = p.cols % VN == 0 && (p.ldx * sizeof(T)) % 16 == 0 && p.ldq % 8 == 0 && aligned(p.x, 16) &&
                    aligned(p.codes, 8);
   auto grid = [&](int rows_per_cta) { return dim3(static_cast<unsigned>((p.rows + rows_per_cta - 1) / rows_per_cta)); };
-  if (!vec || vectors > 4096) return launch_overlapped(quantize_tokens_any_kernel<T>, grid(1), dim3(256), 0, st, p);
+  if (!vec) return launch_overlapped(quantize_tokens_any_kernel<T>, grid(1), dim3(256), 0, st, p);
   if (vectors <= 32) return launch_overlapped(quantize_tokens_kernel<T, 32, 1>, grid(8), dim3(256), 0, st, p);
   if (vectors <= 128) return launch_overlapped(quantize_tokens_kernel<T, 32, 4>, grid(8), dim3(256), 0, st, p);
   if (vectors <= 256) return launch_overlapped(quantize_tokens_kernel<T, 64, 4>, grid(4), dim3(256), 0, st, p);
   if (vectors <= 512) return launch_overlapped(quantize_tokens_kernel<T, 128, 4>, grid(2), dim3(256), 0, st, p);
   if (vectors <= 1024) return launch_overlapped(quantize_tokens_kernel<T, 256, 4>, grid(1), dim3(256), 0, st, p);
   if (vectors <= 2048) return launch_overlapped(quantize_tokens_kernel<T, 512, 4>, grid(1), dim3(512), 0, st, p);
-  return launch_overlapped(quantize_tokens_kernel<T, 512, 8>, grid(1), dim3(512), 0, st, p);
+  return launch_overlapped(quantize_tokens_long_kernel<T>, grid(1), dim3(256), 0, st, p);
 }
 
 // =============================================================================================

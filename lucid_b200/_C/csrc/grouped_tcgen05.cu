@@ -397,10 +397,30 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   const int kb0 = CG == 2 ? 0 : static_cast<int>(static_cast<int64_t>(num_kb) * rank / p.split);
   const int kb1 = CG == 2 ? num_kb : static_cast<int>(static_cast<int64_t>(num_kb) * (rank + 1) / p.split);
 
-  // Warp 0 sets up the barriers and the tile table and, in the split form, requests the first weights before the
-  // rest of the CTA is ready (its copies touch no barrier but this CTA's own); warp 1 allocates TMEM meanwhile.
+  // Warp 0 sets up the barriers and the tile table and requests the first weights: with early_weights before the
+  // codes are there, and in the split form before the rest of the CTA is ready (its copies touch no barrier but this
+  // CTA's own).  Warp 1 allocates TMEM meanwhile.
   uint32_t armed = 0, armed_parity = 0;  // producer: stages with copies in flight, one bit each
   int ahead = 0;                         // producer: stages whose weights have been requested
+  auto request_first = [&]() {
+    if (unit >= s_start[p.E] || p.wait_test) return;
+    TileWalk walk(s_start, s_off, tiles_n, p);
+    const Tile tile = walk.at(unit);
+    const int mine = (tile.rows + C::kStep - 1) / C::kStep * C::kStep / CG;
+    const int boxed = mine == p.tokens / CG ? mine : (mine + C::kBox - 1) / C::kBox * C::kBox;
+    const int n0 = static_cast<int>(tile.n0) + (CG == 2 ? static_cast<int>(rank) * (p.tile_rows / 2) : 0);
+    ahead = min(stages, kb1 - kb0);
+    if (elect_one())
+      for (int s = 0; s < ahead; ++s) {
+        if (CG == 1 || leader) mbar_expect_tx(full_bar(s), static_cast<uint32_t>((p.tile_rows + CG * boxed) * BK));
+        if constexpr (CG == 2)
+          tma_load_3d_pair(tiles_base + s * stage_bytes, &tmap_w, (kb0 + s) * BK, n0, tile.e, map_to_cta(full_bar(s), 0));
+        else
+          tma_load_3d(tiles_base + s * stage_bytes, &tmap_w, (kb0 + s) * BK, n0, tile.e, full_bar(s));
+      }
+    __syncwarp();
+    if (CG == 1 || leader) armed = (1u << ahead) - 1;
+  };
   if (warp == 0) {
     if (lane < MAX_STAGES) {
       mbar_init(full_bar(lane), 1);
@@ -454,21 +474,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     // arrive before the copies are issued: the release of the arrival waits for them otherwise (measured: 4 us)
     __syncwarp();
     cluster_arrive();
-    if (CG == 1 && unit < s_start[p.E] && !p.wait_test) {
-      TileWalk walk(s_start, s_off, tiles_n, p);
-      const Tile tile = walk.at(unit);
-      const int n0 = static_cast<int>(tile.n0), boxes = (tile.rows + C::kBox - 1) / C::kBox;
-      const uint32_t bytes = static_cast<uint32_t>((p.tile_rows + boxes * C::kBox) * BK);
-      ahead = min(stages, kb1 - kb0);
-      if (elect_one())
-        for (int s = 0; s < ahead; ++s) {
-          mbar_expect_tx(full_bar(s), bytes);
-          tma_load_3d(tiles_base + s * stage_bytes, &tmap_w, (kb0 + s) * BK, n0, tile.e, full_bar(s));
-        }
-      __syncwarp();
-      armed = (1u << ahead) - 1;
-    }
-    __syncwarp();
+    if (CG == 1) request_first();
   } else if (warp == 1) {
     if constexpr (CG == 2) {
       asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)),
@@ -501,6 +507,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     int stage = 0;
     uint32_t phase = 0, slot = tiles_base;
     bool ok = true;
+    if (CG == 2) request_first();     // (signals the leader's barriers: not before the cluster has set them up)
     if (p.early_weights) pdl_wait();  // the codes are the previous kernel's
     TileWalk walk(s_start, s_off, tiles_n, p);
     for (int t = unit; t < total && ok && !p.wait_test; t += units) {
@@ -529,7 +536,7 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         }
       };
       int kb = kb0;
-      if (CG == 1 && t == unit && ahead) {  // the first stages have their weights under way
+      if (t == unit && ahead) {  // the first stages have their weights under way
         if (elect_one())
           for (int s = 0; s < ahead; ++s) load_q(s, tiles_base + s * stage_bytes + A_BYTES, kb0 + s);
         __syncwarp();

@@ -87,7 +87,8 @@ def pack_weight(codes: torch.Tensor) -> torch.Tensor:
     if len(strides) < 2:
         raise ValueError("weight codes must have at least two dimensions [N, K]")
     k = codes.shape[-1]
-    if strides[-1] == 1 and strides[-2] >= k and not any(s & 15 for s in strides[:-1]) and codes.data_ptr() & 15 == 0:
+    if (strides[-1] == 1 and strides[-2] >= k and not strides[-2] & 15 and codes.data_ptr() & 15 == 0
+            and (len(strides) == 2 or not any(s & 15 for s in strides[:-2]))):
         return codes
     store = codes.new_zeros((*codes.shape[:-1], (k + 15) // 16 * 16))
     store[..., :k] = codes
@@ -223,7 +224,7 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Ten
     [tokens * top_k, K] (the result of an earlier ``expert_linear``).  ``weight`` [E, N, K] int8 codes
     (see :func:`pack_weight`), ``weight_scale`` and ``bias`` [E, N]; ``activation`` and ``out_dtype`` as
     for :func:`linear`.  The result has ``tokens * top_k`` rows in expert order; rows that belong to no
-    expert are zero, and what ``x`` holds there is not read."""
+    expert are zero, and what ``x`` holds there does not matter."""
     if weight.dim() != 3:
         raise ValueError(f"weight must be [num_experts, N, K], got {tuple(weight.shape)}")
     e, n, k = weight.shape
