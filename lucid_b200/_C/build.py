@@ -1,5 +1,6 @@
-"""Builds liblucid_cuda.so (sm_100a) next to this file with nvcc, and the small CPython module
-``_fastcall`` (gcc) that binds a few of its entry points without ctypes' per-call cost.
+"""Builds liblucid_cuda.so (sm_100a) next to this file with nvcc, and two small CPython modules that spare
+eager calls the host time of ctypes and Python: ``_fastcall`` (gcc, no dependency) binds a few entry points,
+``_torchcall`` (g++ against torch's headers) checks and allocates for the functional operators.
 
     python -m lucid_b200._C.build [--force]
 
@@ -23,6 +24,9 @@ OBJ_DIR = os.path.join(HERE, "build")
 LIB_PATH = os.path.join(HERE, "liblucid_cuda.so")
 FASTCALL_SRC = os.path.join(CSRC, "fastcall.c")
 FASTCALL_PATH = os.path.join(HERE, "_fastcall" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+
+TORCHCALL_SRC = os.path.join(CSRC, "torchcall.cpp")
+TORCHCALL_PATH = os.path.join(HERE, "_torchcall" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 SOURCES = ["api.cu", "quant_kernels.cu", "hist_kernels.cu", "embed_kernels.cu", "qlinear_tcgen05.cu", "wo_kernels.cu",
            "wo_prep_kernels.cu", "peer_kernels.cu", "qgemv_kernels.cu", "grouped_tcgen05.cu", "expert_kernels.cu"]
@@ -80,6 +84,20 @@ def build(force: bool = False, verbose: bool = False) -> str:
             raise RuntimeError("gcc not found; the _fastcall module cannot be built")
         run([cc, "-O2", "-shared", "-fPIC", "-Wall", "-I", sysconfig.get_paths()["include"], "-I", INCLUDE,
              FASTCALL_SRC, "-o", FASTCALL_PATH])
+    if force or not _newer(TORCHCALL_PATH, [TORCHCALL_SRC, os.path.join(INCLUDE, "lucid_cuda.h")]):
+        import torch
+        from torch.utils import cpp_extension
+
+        cxx = shutil.which("g++") or shutil.which("c++")
+        if cxx is None:
+            raise RuntimeError("g++ not found; the _torchcall module cannot be built")
+        lib_dir = os.path.join(os.path.dirname(torch.__file__), "lib")
+        cuda_include = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc))), "include")
+        run([cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", sysconfig.get_paths()["include"],
+             *[f"-isystem{d}" for d in cpp_extension.include_paths()], f"-isystem{cuda_include}", "-I", INCLUDE,
+             TORCHCALL_SRC, "-o", TORCHCALL_PATH, "-L", lib_dir, "-lc10", "-lc10_cuda", "-ltorch_cpu",
+             "-ltorch_python"])
     return LIB_PATH
 
 

@@ -22,6 +22,19 @@ _combine_experts = entry("combine_experts")
 _wo_linear_s8_ex = entry("wo_linear_s8_ex")
 _wo_swiglu_s8_ex = entry("wo_swiglu_s8_ex")
 
+# The functional operators' ordinary calls, checked and allocated natively (see csrc/torchcall.cpp); None when the
+# module has not been built, and the Python forms below serve every call.
+try:
+    from . import _torchcall as torchcall
+except ImportError:
+    torchcall = None
+else:
+    import ctypes as _ctypes
+
+    for _name in ("lc_expert_linear", "lc_expert_linear_workspace_bytes", "lc_route_experts",
+                  "lc_route_experts_workspace_bytes", "lc_combine_experts"):
+        torchcall.bind(_name, _ctypes.cast(getattr(lib, _name), _ctypes.c_void_p).value)
+
 _DTYPE = {
     torch.float32: LC_F32,
     torch.bfloat16: LC_BF16,

@@ -71,7 +71,7 @@ class ExpertRouting:
 
     @property
     def rows(self) -> int:
-        return self.positions.shape[0] * self.positions.shape[1]
+        return self.positions.numel()
 
     def __repr__(self) -> str:
         return f"ExpertRouting(tokens={self.tokens}, top_k={self.top_k}, num_experts={self.num_experts})"
@@ -144,6 +144,20 @@ def _check_cuda(x: torch.Tensor, device: torch.device) -> None:
         raise RuntimeError(f"tensors on different devices: {x.device} and {device}")
 
 
+def _native():
+    """The native forms of the ordinary calls (see ``_C/csrc/torchcall.cpp``), or None.  They return None for a call
+    they do not serve -- the Python form then converts or refuses -- and an int for a failed one."""
+    return getattr(_backend.ops(), "torchcall", None)
+
+
+def _done(result):
+    if type(result) is int:
+        from lucid_b200._C import check
+
+        check(result)
+    return result
+
+
 def _matrix(weight: torch.Tensor) -> tuple:
     shape = weight.shape
     if len(shape) != 2:
@@ -168,6 +182,11 @@ def linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bi
     rows; the result has N / 2 columns).  ``residual`` has the result's shape and is added after the
     activation.  The result has ``out_dtype`` (default: the type of ``x``), which ``residual`` must
     have too."""
+    native = _native()
+    if native is not None:
+        y = native.product(x, weight, weight_scale, bias, _ACTIVATION_ID.get(activation, -1), residual, out_dtype, None, None)
+        if y is not None:
+            return _done(y)
     n, k = _matrix(weight)
     shape = x.shape
     if not shape or shape[-1] != k:
@@ -199,6 +218,13 @@ def route_experts(logits: torch.Tensor, top_k: int, *, renormalize: bool = True)
     A logit of ``-inf`` or NaN is never chosen and carries no weight: a token whose row is all ``-inf``
     (padding) goes nowhere.  Logits of ``+inf`` share the weight evenly.  At most 1024 experts and a
     ``top_k`` of 32."""
+    native = _native()
+    if native is not None:
+        made = native.route(logits, top_k, renormalize)
+        if made is not None:
+            routing = ExpertRouting.__new__(ExpertRouting)
+            routing.weights, routing.experts, routing.offsets, routing.positions = _done(made)
+            return routing
     if logits.dim() != 2:
         raise ValueError(f"logits must be [tokens, num_experts], got {tuple(logits.shape)}")
     if logits.dtype not in _FLOATS:
@@ -225,6 +251,12 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Ten
     (see :func:`pack_weight`), ``weight_scale`` and ``bias`` [E, N]; ``activation`` and ``out_dtype`` as
     for :func:`linear`.  The result has ``tokens * top_k`` rows in expert order; rows that belong to no
     expert are zero, and what ``x`` holds there does not matter."""
+    native = _native()
+    if native is not None:
+        y = native.product(x, weight, weight_scale, bias, _ACTIVATION_ID.get(activation, -1), None, out_dtype,
+                           routing.rows if sorted_rows else routing.positions, routing.offsets)
+        if y is not None:
+            return _done(y)
     if weight.dim() != 3:
         raise ValueError(f"weight must be [num_experts, N, K], got {tuple(weight.shape)}")
     e, n, k = weight.shape
@@ -256,6 +288,11 @@ def combine_experts(y: torch.Tensor, routing: ExpertRouting, *, residual: torch.
     """Brings the experts' rows ``y`` [tokens * top_k, N] back to their tokens: ``out[t] = sum_j
     weights[t, j] * y[positions[t, j]] + residual[t]``, added in the order of j in fp32 and rounded once
     to the type of ``y``, which ``residual`` [tokens, N] must have too."""
+    native = _native()
+    if native is not None:
+        out = native.combine(y, routing.weights, routing.positions, residual)
+        if out is not None:
+            return _done(out)
     if y.dim() != 2 or y.shape[0] != routing.rows:
         raise ValueError(f"y has shape {tuple(y.shape)}, expected ({routing.rows}, N)")
     device = y.device

@@ -576,3 +576,66 @@ def test_waits_that_run_out_leave_a_status(ops, variant):
     y = ops.grouped_qlinear_i8(q, w, one[:1], one, variant=variant)  # the GPU keeps working
     want = (q.cpu().numpy().astype(np.int64) @ w.cpu().numpy().astype(np.int64).T).astype(np.float32)
     np.testing.assert_array_equal(y.cpu().numpy(), want)
+
+
+# ---- the native form of ordinary calls -----------------------------------------------------------------
+def test_native_and_python_forms_agree(F, ops, monkeypatch):
+    assert ops.torchcall is not None, "lucid_b200/_C/_torchcall was not built"
+    g = generator(21)
+    x = torch.randn(48, 96, generator=g, device="cuda").bfloat16()
+    w, sw = make_weight(g, 64, 96)
+    we, se = make_weight(g, 5, 64, 96)
+    res, bias = torch.randn(48, 64, generator=g, device="cuda").bfloat16(), torch.randn(64, generator=g, device="cuda")
+    logits = torch.randn(48, 5, generator=g, device="cuda")
+
+    def calls():
+        r = F.route_experts(logits, 2, renormalize=False)
+        h = F.expert_linear(x, we, se, r, activation="silu", out_dtype=torch.float16)
+        y = F.expert_linear(h[:, :64].contiguous(), we[:, :, :64].contiguous(), se, r, sorted_rows=True)
+        return [r.weights, r.experts, r.offsets, r.positions, h, y, F.combine_experts(y, r), F.linear(x, w, sw),
+                F.linear(x, w, sw, bias, activation="gelu", residual=res),
+                F.linear(x, w, sw, activation="swiglu", out_dtype=torch.float32)]
+
+    native = calls()
+    monkeypatch.setattr(ops, "torchcall", None)
+    for a, b in zip(native, calls()):
+        assert a.dtype == b.dtype and a.shape == b.shape and torch.equal(a, b)
+    monkeypatch.undo()
+    t = ops.torchcall
+    # calls that are not ordinary are left to the Python form
+    assert t.product(x[:, ::2], w[:, :48], sw, None, 0, None, None, None, None) is None      # strided rows
+    assert t.product(x, w, sw.double(), None, 0, None, None, None, None) is None             # another type
+    assert t.product(x, w, sw, None, 7, None, None, None, None) is None                      # no such activation
+    assert t.product(x, w, sw, None, 0, res.float(), None, None, None) is None               # residual of another type
+    assert t.product(x, w[:, :90], sw, None, 0, None, None, None, None) is None              # does not contract
+    assert t.product(x[:0], w, sw, None, 0, None, None, None, None) is None                  # empty
+    assert t.product(x.cpu(), w, sw, None, 0, None, None, None, None) is None
+    assert t.route(logits, 6, True) is None and t.route(logits[:0], 2, True) is None
+    assert t.combine(native[5][:90], native[0], native[3], None) is None
+    with pytest.raises(TypeError):
+        t.product(x)
+
+
+def test_calls_from_another_stream_and_thread(F):
+    """Calls of two host threads on two streams at once."""
+    import threading
+
+    g = generator(33)
+    w, sw = make_weight(g, 512, 1024)
+    xs = [torch.randn(40, 1024, generator=g, device="cuda") for _ in range(2)]
+    want = [F.linear(x, w, sw, activation="gelu") for x in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i].append(F.linear(xs[i], w, sw, activation="gelu"))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(y, want[i]) for i in range(2) for y in got[i])
