@@ -304,7 +304,7 @@ int32_t lc_dynamic_linear_f32(const float* x, int64_t ldx, int64_t M, int64_t K,
  *   out[m,n] = act(f32(acc - zx*wsum[e,n]) * (sx[m] * sw[e,n]) + bias[e,n]) + residual[m,n],
  *   acc      = sum_k q[m,k] * wq[e,n,k]  (int32, exact),  e = the group whose rows contain m.
  * q [rows, ldq]: int8 (or uint8, q_unsigned) codes, rows sorted by group; offsets [groups + 1] on the device:
- * group e owns rows offsets[e] .. offsets[e+1] (ascending; values are clamped to [0, rows]).  offsets NULL:
+ * group e owns rows offsets[e] .. offsets[e+1] (values are clamped to [0, rows] and to ascending order).  offsets NULL:
  * one group of all rows, the dense Linear.  Rows behind the last group's come out as zeros.
  * wq [groups, N, ldw] with group_stride elements between groups; sw / bias / wsum [groups, N]; sx one value or
  * one per row (sx_per_row); zx a device scalar, together with wsum, or both NULL.

@@ -46,8 +46,8 @@ struct Vec16 {
 // One warp per token: lane l holds the EPL values l*EPL .. l*EPL + EPL-1 in registers and their maximum.  A round is
 // one warp-wide integer maximum (order-preserving bits of the value) and a vote: of several lanes with the largest
 // value the lowest has the lowest expert, and that lane moves on to its next one.  Up to four values a lane are
-// sorted first, so that moving on is a shift (16384 x 128, 8 of them: 538 -> TODO instructions a token, which is what
-// the kernel is bound by); more are searched.
+// sorted first, so that moving on is a shift; more are searched.  The kernel is bound by the instructions of a token
+// (16384 tokens of 128 experts, 8 of them chosen: 498), 16.8 us together with the second kernel's latency.
 // A warp walks a contiguous run of tokens and counts its choices per expert in shared memory; a choice's
 // count is its rank inside the run.  Small batches (one CTA) finish in the same kernel; otherwise each CTA
 // leaves its counts and its ranks, and the second kernel adds what precedes them.  Every sum is an integer

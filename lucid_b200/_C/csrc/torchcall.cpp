@@ -84,7 +84,7 @@ PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   const int64_t e = experts ? w->size(0) : 0, n = w->size(lead), k = w->size(lead + 1), ldw = w->stride(lead);
   const int64_t stride = experts ? w->stride(0) : 0;
   if (k != x->size(1) || k < 1 || n < 1 || w->stride(lead + 1) != 1 || ldw < k || ldw % 16 || stride % 16 ||
-      reinterpret_cast<uintptr_t>(w->data_ptr()) % 16)
+      (e > 1 && stride < n * ldw) || reinterpret_cast<uintptr_t>(w->data_ptr()) % 16)
     return none();
   const long act = PyLong_AsLong(args[4]);
   if (act < LC_ACT_NONE || act > LC_ACT_SWIGLU || (act == LC_ACT_SWIGLU && n % 16)) return PyErr_Occurred() ? nullptr : none();

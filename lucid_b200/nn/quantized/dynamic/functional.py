@@ -15,6 +15,9 @@ Nothing of the routing is read on the host, so the calls can be captured in a CU
 dynamically quantized layers themselves these are inference functions: results carry no gradient.
 All tensors are CUDA tensors of one device; calls go to its current stream.  The reference has no
 counterpart of this module (its dynamic Linear is ``lucid/nn/quantized/dynamic/linear.py:85-92``).
+
+As in the framework's quantizer a NaN in an activation row counts as zero; an infinity makes the
+row's results NaN.
 """
 from __future__ import annotations
 
@@ -87,9 +90,11 @@ def pack_weight(codes: torch.Tensor) -> torch.Tensor:
     if len(strides) < 2:
         raise ValueError("weight codes must have at least two dimensions [N, K]")
     k = codes.shape[-1]
-    if (strides[-1] == 1 and strides[-2] >= k and not strides[-2] & 15 and codes.data_ptr() & 15 == 0
-            and (len(strides) == 2 or not any(s & 15 for s in strides[:-2]))):
-        return codes
+    if strides[-1] == 1 and strides[-2] >= k and not strides[-2] & 15 and codes.data_ptr() & 15 == 0:
+        # (of several matrices: whole ones behind one another)
+        if len(strides) == 2 or (len(strides) == 3 and not strides[0] & 15
+                                 and (codes.shape[0] == 1 or strides[0] >= codes.shape[1] * strides[1])):
+            return codes
     store = codes.new_zeros((*codes.shape[:-1], (k + 15) // 16 * 16))
     store[..., :k] = codes
     return store[..., :k]

@@ -96,6 +96,8 @@ def share_quantized_input():
 
 
 class Linear(nn.Module):
+    activation: str | None = None  # see set_activation (a class attribute: older pickles have none of their own)
+
     def __init__(self, in_features: int, out_features: int, bias: bool = True) -> None:
         super().__init__()
         self.in_features = in_features
@@ -104,7 +106,6 @@ class Linear(nn.Module):
         self.act_qdtype: QDtype = quint8
         self.act_scheme = "tensor_affine"
         self.out_dtype = torch.float32
-        self.activation: str | None = None
         self.register_buffer("weight_int8", torch.zeros((out_features, in_features), dtype=torch.int8))
         self.register_buffer("weight_scale", torch.ones(out_features))
         self.register_buffer("weight_zero_point", torch.zeros(out_features))

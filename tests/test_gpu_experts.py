@@ -639,3 +639,110 @@ def test_calls_from_another_stream_and_thread(F):
     for t in threads:
         t.join()
     assert all(torch.equal(y, want[i]) for i in range(2) for y in got[i])
+
+
+# ---- calls the documentation allows and nothing above makes --------------------------------------------
+def test_offsets_out_of_order_are_made_ascending(ops):
+    """Nothing outside is read or written and every row is computed at most once, whatever the offsets hold."""
+    g = generator(8)
+    rows, n, k = 300, 64, 64
+    q = torch.randint(-128, 128, (rows, k), generator=g, device="cuda").to(torch.int8)
+    w = torch.randint(-128, 128, (40, n, k), generator=g, device="cuda").to(torch.int8)
+    one = torch.ones(40, n, device="cuda")
+    raw = torch.randint(-50, 400, (41,), generator=g, device="cuda", dtype=torch.int32)
+    ends = torch.cummax(raw.clamp(0, rows), 0).values.tolist()
+    for variant in range(7):
+        y = ops.grouped_qlinear_i8(q, w, one[0, :1], one, offsets=raw, variant=variant)
+        want = np.zeros((rows, n), np.float32)
+        for e in range(40):
+            a, b = ends[e], ends[e + 1]
+            want[a:b] = q[a:b].cpu().numpy().astype(np.int64) @ w[e].cpu().numpy().astype(np.int64).T
+        got = y.cpu().numpy()
+        np.testing.assert_array_equal(got[ends[0]:], want[ends[0]:])  # (rows before the first group are nobody's)
+
+
+def test_weights_that_are_views(F):
+    g = generator(12)
+    base = torch.randint(-128, 128, (6, 48, 96), generator=g, device="cuda").to(torch.int8)
+    sw = 0.002 * (0.5 + torch.rand(6, 48, generator=g, device="cuda"))
+    r = F.route_experts(torch.randn(20, 6, generator=g, device="cuda"), 2)
+    x = torch.randn(20, 64, generator=g, device="cuda")
+    for view in (base[:, :, 16:80], base[:, ::2, :64].repeat_interleave(2, 1), base[:1, :, :64].expand(6, 48, 64),
+                 base.transpose(0, 1).contiguous().transpose(0, 1)[:, :, :64], base[..., 1:65]):
+        got = F.expert_linear(x, view, sw, r)
+        assert torch.equal(got, F.expert_linear(x, view.contiguous(), sw, r))
+
+
+def test_values_that_are_not_numbers(F):
+    g = generator(14)
+    w, sw = make_weight(g, 64, 128)
+    x = torch.randn(4, 128, generator=g, device="cuda")
+    x[1, 5] = math.nan
+    x[2, 7] = -math.inf
+    clean = x.clone()
+    clean[1, 5] = 0.0
+    for activation in (None, "relu", "gelu", "gelu_tanh", "silu", "swiglu"):
+        y = F.linear(x, w, sw, activation=activation)
+        assert torch.equal(y[[0, 1, 3]], F.linear(clean, w, sw, activation=activation)[[0, 1, 3]])
+        assert y[2].isnan().all()
+
+
+def test_one_row_in_all_experts_and_many_experts(F):
+    g = generator(15)
+    w, sw = make_weight(g, 1024, 16, 32)
+    x = torch.randn(3, 32, generator=g, device="cuda").half()
+    r = F.route_experts(torch.randn(3, 1024, generator=g, device="cuda"), 32)
+    y = F.expert_linear(x, w, sw, r)
+    q, s = plain_codes(x)
+    experts, positions = r.experts.cpu().numpy(), r.positions.cpu().numpy()
+    for t in range(3):
+        for j in range(32):
+            e = experts[t, j]
+            want, err = plain_product(q[t:t + 1], s[t:t + 1], w[e].cpu().numpy(), f64(sw[e]), None, None)
+            check(y[positions[t, j]][None], want, err, torch.float16)
+
+
+def test_first_call_of_a_process_inside_a_capture():
+    """Nothing the operators set up on their first call disturbs a graph capture."""
+    import os
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from lucid_b200.nn.quantized.dynamic import functional as F
+x = torch.randn(5, 64, device="cuda"); logits = torch.randn(5, 4, device="cuda")
+w = torch.randint(-9, 9, (4, 64, 64), device="cuda").to(torch.int8); s = torch.ones(4, 64, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    r = F.route_experts(logits, 2)
+    y = F.combine_experts(F.expert_linear(x, w, s, r, activation="silu"), r)
+graph.replay()
+r2 = F.route_experts(logits, 2)
+assert torch.equal(y, F.combine_experts(F.expert_linear(x, w, s, r2, activation="silu"), r2))
+print("same")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=root, timeout=300)
+    assert done.returncode == 0 and "same" in done.stdout, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("rows", [70000])
+def test_offsets_beyond_32_bits(F, rows):
+    """Elements of the input and the result past 2^31."""
+    g = generator(16)
+    k, n = 32784, 32
+    x = torch.empty(rows, k, dtype=torch.bfloat16, device="cuda")
+    assert x.numel() > 2 ** 31
+    tail = torch.randn(3, k, generator=g, device="cuda").bfloat16()
+    x[:-3] = 0
+    x[-3:] = tail
+    w, sw = make_weight(g, n, k)
+    y = F.linear(x, w, sw)
+    assert torch.equal(y[-3:], F.linear(tail, w, sw)) and (y[:-3] == 0).all()
+    wide, wsw = make_weight(g, 40960, 64)
+    small = torch.randn(53000, 64, generator=g, device="cuda").bfloat16()
+    big = F.linear(small, wide, wsw)
+    assert big.numel() > 2 ** 31
+    assert torch.equal(big[-5:], F.linear(small[-5:], wide, wsw))
