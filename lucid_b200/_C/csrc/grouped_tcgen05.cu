@@ -17,7 +17,7 @@
 // Two forms:
 //  * pair (cta_group::2): 256 weight rows x up to 256 rows of q per tile, each CTA of the pair loading
 //    its own 128 weight rows and half of the q rows; for groups that fill such tiles.
-//  * split (cta_group::1): 128 weight rows x up to 16 or 64 rows of q, K cut over the CTAs of a cluster.
+//  * split (cta_group::1): 128 weight rows x up to 64 rows of q, K cut over the CTAs of a cluster.
 //    Decode batches have few tiles (a [4096, 14336] layer: 32), and a cluster of up to eight gives every
 //    SM a share of the weight's bytes.  The partial sums are int32, so adding them in rank 0's shared
 //    memory in any order gives the same bits.
@@ -223,29 +223,51 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either i
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-// v * Phi(v) = max(v, 0) - a Phi(-a), a = |v|, Phi the normal distribution function.  Phi(-a) = 2^p(a), p a polynomial
-// of degree 9 fitted to log2 Phi(-a) on [0, 6] (least squares over Chebyshev nodes, reweighted towards the smallest
-// largest error in a * Phi): a * Phi(-a) is off by at most 3.5e-8, and by 2e-12 beyond 6.  13 instructions where the
-// library's erff takes about 40: an 8192 x 2048 x 512 product, whose time is the epilogue's, 24.7 us against 32.3 us.
-__device__ __forceinline__ float gelu(float v) {
-  const float a = fminf(fabsf(v), 10.0f);
-  float p = 2.9685912750210264e-07f;
-  p = fmaf(p, a, -6.425118044717237e-06f);
-  p = fmaf(p, a, 5.635188063024543e-05f);
-  p = fmaf(p, a, -0.00022571126464754343f);
-  p = fmaf(p, a, -9.095141285797581e-05f);
-  p = fmaf(p, a, 0.007042091339826584f);
-  p = fmaf(p, a, -0.052499450743198395f);
-  p = fmaf(p, a, -0.4592026472091675f);
-  p = fmaf(p, a, -1.151106357574463f);
-  p = fmaf(p, a, -0.9999999403953552f);
-  return fmaf(-a, exp2_approx(p), max_nan(v, 0.0f));
+// two fp32 values in one register pair: one instruction multiplies or multiply-adds both
+struct Pair {
+  unsigned long long v;
+};
+__device__ __forceinline__ Pair pack(float lo, float hi) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack(Pair a, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v));
+}
+__device__ __forceinline__ Pair mul(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+// v * Phi(v) = max(v, 0) - |v| Phi(-|v|), Phi the normal distribution function, for two values.  Phi(n) = 2^p(n) for
+// n = -|v|, p a polynomial of degree 9 fitted to log2 Phi on [-6, 0] (least squares over Chebyshev nodes, reweighted
+// towards the smallest largest error in n * Phi): n * Phi(n) is off by at most 3.5e-8, and by 2e-12 beyond -6.  20
+// instructions a pair where the library's erff takes about 80: an 8192 x 2048 x 512 product, whose time is the
+// epilogue's, 24.0 us against 32.3 us.
+__device__ __forceinline__ void gelu(float& v0, float& v1) {
+  const float n0 = fmaxf(-fabsf(v0), -10.0f), n1 = fmaxf(-fabsf(v1), -10.0f);
+  const Pair n = pack(n0, n1);
+  constexpr float kCoeff[10] = {-2.9685912750210264e-07f, -6.425118044717237e-06f, -5.635188063024543e-05f,
+                                -0.00022571126464754343f, 9.095141285797581e-05f,  0.007042091339826584f,
+                                0.052499450743198395f,    -0.4592026472091675f,    1.151106357574463f,
+                                -0.9999999403953552f};
+  Pair p = pack(kCoeff[0], kCoeff[0]);
+#pragma unroll
+  for (int i = 1; i < 10; ++i) p = fma(p, n, pack(kCoeff[i], kCoeff[i]));
+  float p0, p1;
+  unpack(p, p0, p1);
+  unpack(fma(n, pack(exp2_approx(p0), exp2_approx(p1)), pack(max_nan(v0, 0.0f), max_nan(v1, 0.0f))), v0, v1);
 }
 
 template <int ACT>
 __device__ __forceinline__ float activate(float v) {
   if constexpr (ACT == LC_ACT_RELU) return v < 0.0f ? 0.0f : v;  // NaN compares false and stays
-  if constexpr (ACT == LC_ACT_GELU) return gelu(v);
   if constexpr (ACT == LC_ACT_GELU_TANH)  // 0.5 v (1 + tanh(u)) = v / (1 + exp(-2u)), u = sqrt(2/pi) (v + 0.044715 v^3)
     return sigmoid_times(v, 1.5957691216057307f * (v + 0.044715f * v * v * v));
   if constexpr (ACT == LC_ACT_SILU) return sigmoid_times(v, v);
@@ -295,6 +317,7 @@ __device__ __forceinline__ void drain(const Params& p, const Lane& l) {
   const int64_t col = ACT == LC_ACT_SWIGLU ? (((l.n >> 4) << 3) | (l.n & 7)) : l.n;
   const int64_t row0 = l.m0 + (ACT == LC_ACT_SWIGLU ? up : 0);
   const T* const res = static_cast<const T*>(p.residual);
+  const Pair sw2 = pack(l.sw, l.sw), bias2 = pack(l.bias, l.bias);
 #pragma unroll 1
   for (int c = l.first; c < l.rows; c += EPI_WARPS / 4 * CH) {
     const int left = l.in ? l.rows - c : 0;
@@ -329,9 +352,13 @@ __device__ __forceinline__ void drain(const Params& p, const Lane& l) {
 #pragma unroll
     for (int j = 0; j < CH; j += 4) {
       const float4 s = *reinterpret_cast<const float4*>(l.sx + c + j);
-      const float sv[4] = {s.x, s.y, s.z, s.w};
+      auto value = [&](int i) { return static_cast<float>(static_cast<int>(r[i])); };
+      unpack(fma(pack(value(j), value(j + 1)), mul(pack(s.x, s.y), sw2), bias2), f[j], f[j + 1]);
+      unpack(fma(pack(value(j + 2), value(j + 3)), mul(pack(s.z, s.w), sw2), bias2), f[j + 2], f[j + 3]);
+    }
+    if constexpr (ACT == LC_ACT_GELU) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) f[j + i] = fmaf(static_cast<float>(static_cast<int>(r[j + i])), sv[i] * l.sw, l.bias);
+      for (int j = 0; j < CH; j += 2) gelu(f[j], f[j + 1]);
     }
     T* o = static_cast<T*>(p.out) + (row0 + c) * p.ldo + col;
     auto finish = [&](int j) {  // the result of row c + j
