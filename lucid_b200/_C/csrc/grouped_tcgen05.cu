@@ -991,7 +991,7 @@ static int32_t check_and_launch(const char* what, const void* q, int q_unsigned,
                                 int64_t N, int64_t K, const float* sx, int sx_per_row, const float* zx,
                                 const int32_t* wsum, const float* sw, const float* bias, int act, const void* residual,
                                 int64_t ldr, void* out, int out_dtype, int64_t ldo, int32_t* status, int variant,
-                                int early_weights, cudaStream_t st) {
+                                int early_weights, bool only_check, cudaStream_t st) {
   const int wait_test = (variant & LC_QLINEAR_WAIT_TEST) ? 1 : 0;
   variant &= ~LC_QLINEAR_WAIT_TEST;
   if (wait_test && !status) return fail(LC_ERR_INVALID_ARG, "%s: the wait test needs a status word", what);
@@ -1015,6 +1015,7 @@ static int32_t check_and_launch(const char* what, const void* q, int q_unsigned,
   // |sum| <= K * 255 * 128 must stay inside int32; rows and columns inside the TMA coordinate range
   if (K > 65536) return fail(LC_ERR_UNSUPPORTED, "%s: K above 65536 could overflow int32", what);
   if (R > 0x7fffffffLL - 512 || N > 0x7fffffffLL - 512) return fail(LC_ERR_UNSUPPORTED, "%s: dimension too large", what);
+  if (only_check) return LC_OK;
   Params p = {};
   p.R = R;
   p.N = N;
@@ -1053,7 +1054,7 @@ extern "C" int32_t lc_grouped_qlinear_i8(const void* q, int32_t q_unsigned, int6
                                          void* stream) {
   return grouped::check_and_launch("grouped_qlinear_i8", q, q_unsigned, ldq, rows, offsets, groups, wq, ldw,
                                    group_stride, N, K, sx, sx_per_row, zx, wsum, sw, bias, activation, residual, ldr,
-                                   out, out_dtype, ldo, status, variant, 0, as_stream(stream));
+                                   out, out_dtype, ldo, status, variant, 0, false, as_stream(stream));
 }
 
 // ---- quantization of the activations and the product as one call --------------------------------
@@ -1080,11 +1081,15 @@ extern "C" int32_t lc_expert_linear(const void* x, int32_t x_dtype, int64_t x_ro
                 (long long)lc_expert_linear_workspace_bytes(rows, K));
   uint8_t* codes = static_cast<uint8_t*>(workspace);
   float* scale = reinterpret_cast<float*>(codes + round256(rows * pad16(K)));
+  auto product = [&](bool only_check) {
+    return grouped::check_and_launch("expert_linear", codes, 0, pad16(K), rows, offsets, groups, wq, ldw, group_stride, N, K,
+                                     scale, 1, nullptr, nullptr, sw, bias, activation, residual, ldr, out, out_dtype, ldo,
+                                     status, 0, 1, only_check, as_stream(stream));
+  };
+  if (int32_t rc = product(true)) return rc;  // refused before anything is launched
   if (int32_t rc = lc_quantize_tokens(x, x_dtype, x_rows, K, ldx, positions, top_k, rows,
                                       offsets && !positions ? offsets + groups : nullptr,
                                       reinterpret_cast<int8_t*>(codes), pad16(K), scale, stream))
     return rc;
-  return grouped::check_and_launch("expert_linear", codes, 0, pad16(K), rows, offsets, groups, wq, ldw, group_stride, N,
-                                   K, scale, 1, nullptr, nullptr, sw, bias, activation, residual, ldr, out, out_dtype,
-                                   ldo, status, 0, 1, as_stream(stream));
+  return product(false);
 }

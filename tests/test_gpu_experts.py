@@ -746,3 +746,34 @@ def test_offsets_beyond_32_bits(F, rows):
     big = F.linear(small, wide, wsw)
     assert big.numel() > 2 ** 31
     assert torch.equal(big[-5:], F.linear(small[-5:], wide, wsw))
+
+
+def test_refusals_of_the_library_reach_python(F):
+    from lucid_b200._C import LucidCudaError
+
+    x, w = torch.zeros(2, 65552, device="cuda"), torch.zeros(16, 65552, dtype=torch.int8, device="cuda")
+    with pytest.raises(LucidCudaError, match="overflow"):
+        F.linear(x, w, torch.ones(16, device="cuda"))
+    with pytest.raises(ValueError, match="residual"):
+        F.linear(x[:, :64].contiguous(), w[:, :64], torch.ones(16, device="cuda"), residual=torch.zeros(3, 16, device="cuda"))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        F.linear(torch.zeros(2, 64), w[:, :64].cpu(), torch.ones(16))
+    with pytest.raises(RuntimeError, match="different devices"):
+        F.linear(x[:, :64].contiguous(), w[:, :64].cpu(), torch.ones(16, device="cuda"))
+    ok = F.linear(x[:, :64].contiguous(), w[:, :64], torch.ones(16, device="cuda"))  # and the GPU goes on
+    assert (ok == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantize_rows_of_every_alignment(ops, dtype):
+    """Rows whose start, pitch and length are no multiples of a vector."""
+    g = generator(40)
+    store = torch.randn(64 * 4200, generator=g, device="cuda").to(dtype)
+    for cols, ldx in ((1, 1), (7, 7), (9, 13), (31, 33), (255, 257), (1003, 1003), (1021, 1029), (2049, 2051), (4099, 4101)):
+        for start in (0, 1, 3, 6):
+            rows = min(13, (store.numel() - start) // ldx)
+            x = store[start:].as_strided((rows, cols), (ldx, 1))
+            q, s = ops.quantize_tokens(x)
+            want_q, want_s = plain_codes(x)
+            np.testing.assert_array_equal(q.cpu().numpy().astype(np.int64), want_q)
+            np.testing.assert_array_equal(f64(s), want_s)
