@@ -178,16 +178,27 @@ struct Tile {
   int64_t n0;       // first weight row inside the group
 };
 
-// Tiles are numbered group by group; within a group, bands of 16 row tiles share the weight tiles.  The walk
-// only moves forward because a CTA's tile numbers grow.
+// Tiles are numbered group by group; within a group, bands of 16 row tiles share the weight tiles.  The walk only
+// moves forward, because a CTA's tile numbers grow: to this group's next tile or, by bisection, to a later group (a
+// token among 128 experts leaves 122 empty groups to step over).
 struct TileWalk {
   const int* start;  // [E + 1] first tile of each group
   const int* off;    // [E + 1] first row of each group
-  int tiles_n, tokens, tile_rows, e;
+  int tiles_n, tokens, tile_rows, groups, e;
   __device__ __forceinline__ TileWalk(const int* s, const int* o, int tn, const Params& p)
-      : start(s), off(o), tiles_n(tn), tokens(p.tokens), tile_rows(p.tile_rows), e(0) {}
+      : start(s), off(o), tiles_n(tn), tokens(p.tokens), tile_rows(p.tile_rows), groups(p.E), e(0) {}
   __device__ __forceinline__ Tile at(int t) {
-    while (t >= start[e + 1]) ++e;
+    if (t >= start[e + 1]) {  // the first group behind whose tiles t does not lie
+      int lo = e + 1, hi = groups - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (t >= start[mid + 1])
+          lo = mid + 1;
+        else
+          hi = mid;
+      }
+      e = lo;
+    }
     const int rows = off[e + 1] - off[e];
     const int tiles_m = (rows + tokens - 1) / tokens;
     const int local = t - start[e];
@@ -483,27 +494,37 @@ grouped_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         s_off[0] = top;
         s_start[0] = 0;
       }
-      for (int e0 = 0; e0 < p.E; e0 += 32) {
-        const int e = e0 + lane;
-        int end = e < p.E ? min(max(p.offsets[e + 1], top), R) : top;
+      constexpr int kAtOnce = 4;  // chunks of 32 offsets requested together
+      for (int e1 = 0; e1 < p.E; e1 += 32 * kAtOnce) {
+        int raw[kAtOnce];
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int v = __shfl_up_sync(0xffffffffu, end, o);
-          if (lane >= o) end = max(end, v);
+        for (int i = 0; i < kAtOnce; ++i) {
+          const int e = e1 + i * 32 + lane;
+          raw[i] = e < p.E ? p.offsets[e + 1] : 0;
         }
-        const int before = __shfl_up_sync(0xffffffffu, end, 1);
-        int sum = (end - (lane ? before : top) + p.tokens - 1) / p.tokens * tiles_n;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int v = __shfl_up_sync(0xffffffffu, sum, o);
-          if (lane >= o) sum += v;
+        for (int i = 0; i < kAtOnce; ++i) {
+          const int e = e1 + i * 32 + lane;
+          int end = min(max(raw[i], top), R);
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, end, o);
+            if (lane >= o) end = max(end, v);
+          }
+          const int before = __shfl_up_sync(0xffffffffu, end, 1);
+          int sum = (end - (lane ? before : top) + p.tokens - 1) / p.tokens * tiles_n;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
+          }
+          if (e < p.E) {
+            s_off[e + 1] = end;
+            s_start[e + 1] = base + sum;
+          }
+          base += __shfl_sync(0xffffffffu, sum, 31);
+          top = __shfl_sync(0xffffffffu, end, 31);
         }
-        if (e < p.E) {
-          s_off[e + 1] = end;
-          s_start[e + 1] = base + sum;
-        }
-        base += __shfl_sync(0xffffffffu, sum, 31);
-        top = __shfl_sync(0xffffffffu, end, 31);
       }
     }
     // arrive before the copies are issued: the release of the arrival waits for them otherwise (measured: 4 us)
