@@ -458,7 +458,7 @@ def expert_linear(x2d, wq, sw, bias, positions, offsets, rows: int, activation: 
     return out
 
 
-_ROUTE_ONE_CTA = 128  # tokens up to which lc_route_experts needs no workspace
+_ROUTE_ONE_CTA = 32  # tokens up to which lc_route_experts needs no workspace
 
 
 def route_experts(logits, top_k: int, renormalize: bool):
