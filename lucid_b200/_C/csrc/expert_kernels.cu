@@ -46,8 +46,9 @@ struct Vec16 {
 //
 // One warp per token: lane l holds the EPL values l*EPL .. l*EPL + EPL-1 in registers and their maximum.  A round is
 // one warp-wide integer maximum (order-preserving bits of the value) and a vote: of several lanes with the largest
-// value the lowest has the lowest expert, and that lane moves on to its next one.  Up to four values a lane are
-// sorted first, so that moving on is a shift; more are searched.  The kernel is bound by the instructions of a token
+// value the lowest has the lowest expert, and that lane moves on to its next one.  Up to eight values a
+// lane are sorted first, in lists of up to four, so that moving on is a shift (16384 tokens of 256 experts, 8 of them
+// chosen: 21.3 us, 24.1 with a search for the lane's next value); more are searched.  The kernel is bound by the instructions of a token
 // (16384 tokens of 128 experts, 8 of them chosen: 498), 16.8 us together with the second kernel's latency.
 // A warp walks a contiguous run of tokens and counts its choices per expert in shared memory; a choice's
 // count is its rank inside the run.  Small batches (one CTA) finish in the same kernel; otherwise each CTA
@@ -169,34 +170,47 @@ __global__ void __launch_bounds__(1024) route_kernel(const RouteParams p) {
     // lane j keeps the j-th choice
     uint32_t my_key = 0, best = top;
     int my_e = -1;
-    if constexpr (EPL <= 4) {
-      // descending, equal values in the order of their experts; two bits per value say where it came from
-      uint32_t from = 0xe4u;  // 3, 2, 1, 0
-      auto order = [&](int i) {  // values i and i + 1
-        const bool swap = key[i + 1] > key[i];
-        const uint32_t hi = max(key[i], key[i + 1]), lo = min(key[i], key[i + 1]);
-        key[i] = hi;
-        key[i + 1] = lo;
-        const uint32_t bits = ((from >> 2 * i) ^ (from >> 2 * (i + 1))) & 3u;
-        if (swap) from ^= bits << 2 * i | bits << 2 * (i + 1);
-      };
+    if constexpr (EPL <= 8) {
+      // lists of up to four: descending, equal values in the order of their experts; two bits per value say where it
+      // came from.  Of a lane's two lists with the same head the first has the lower expert.
+      constexpr int LEN = EPL < 4 ? EPL : 4, LISTS = EPL / LEN;
+      uint32_t from[LISTS];
 #pragma unroll
-      for (int n = EPL - 1; n > 0; --n)
+      for (int l = 0; l < LISTS; ++l) {
+        uint32_t* k = key + l * LEN;
+        from[l] = 0xe4u;  // 3, 2, 1, 0
 #pragma unroll
-        for (int i = 0; i < n; ++i) order(i);
+        for (int n = LEN - 1; n > 0; --n)
+#pragma unroll
+          for (int i = 0; i < n; ++i) {
+            const bool swap = k[i + 1] > k[i];
+            const uint32_t hi = max(k[i], k[i + 1]), lo = min(k[i], k[i + 1]);
+            k[i] = hi;
+            k[i + 1] = lo;
+            const uint32_t bits = ((from[l] >> 2 * i) ^ (from[l] >> 2 * (i + 1))) & 3u;
+            if (swap) from[l] ^= bits << 2 * i | bits << 2 * (i + 1);
+          }
+      }
       for (int j = 0; j < K && best; ++j) {
-        const int winner = __ffs(__ballot_sync(0xffffffffu, key[0] == best)) - 1;
-        const int e = __shfl_sync(0xffffffffu, lane * EPL + static_cast<int>(from & 3u), winner);
+        const bool second = LISTS > 1 && key[0] != best;
+        const uint32_t head = second ? key[EPL - LEN] : key[0];
+        const int at = lane * EPL + (second ? LEN + static_cast<int>(from[LISTS - 1] & 3u) : static_cast<int>(from[0] & 3u));
+        const int winner = __ffs(__ballot_sync(0xffffffffu, head == best)) - 1;
+        const int e = __shfl_sync(0xffffffffu, at, winner);
         if (lane == j) {
           my_key = best;
           my_e = e;
         }
         if (lane == winner) {
 #pragma unroll
-          for (int i = 0; i < EPL; ++i) key[i] = i + 1 < EPL ? key[i + 1] : 0u;
-          from >>= 2;
+          for (int l = 0; l < LISTS; ++l) {
+            if (second != (l == 1)) continue;
+#pragma unroll
+            for (int i = 0; i < LEN; ++i) key[l * LEN + i] = i + 1 < LEN ? key[l * LEN + i + 1] : 0u;
+            from[l] >>= 2;
+          }
         }
-        best = __reduce_max_sync(0xffffffffu, key[0]);
+        best = __reduce_max_sync(0xffffffffu, LISTS > 1 ? max(key[0], key[EPL - LEN]) : key[0]);
       }
     } else {
       for (int j = 0; j < K && best; ++j) {

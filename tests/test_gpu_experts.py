@@ -320,6 +320,20 @@ def test_route(F, dtype, tokens, experts, top_k, renormalize):
     np.testing.assert_allclose(r.weights.cpu().numpy(), weights, rtol=48 * 2.0 ** -23, atol=1e-37)
 
 
+@pytest.mark.parametrize("experts,top_k", [(20, 20), (50, 32), (64, 8), (100, 16), (129, 8), (200, 32), (256, 9), (500, 12)])
+def test_route_equal_logits(F, experts, top_k):
+    # three values, so that nearly every choice is among equals; a NaN and a -inf between them
+    logits = torch.randint(0, 3, (70, experts), generator=generator(experts), device="cuda").float()
+    logits[::3, 7] = math.nan
+    logits[::2, 9:12] = -math.inf
+    r = F.route_experts(logits, top_k)
+    weights, chosen, offsets, positions = plain_route(logits, top_k, True)
+    np.testing.assert_array_equal(r.experts.cpu().numpy(), chosen)
+    np.testing.assert_array_equal(r.offsets.cpu().numpy(), offsets)
+    np.testing.assert_array_equal(r.positions.cpu().numpy(), positions)
+    np.testing.assert_allclose(r.weights.cpu().numpy(), weights, rtol=48 * 2.0 ** -23)
+
+
 def test_route_special_logits(F):
     inf, nan, low = math.inf, math.nan, torch.finfo(torch.float32).min
     logits = torch.tensor([[inf, 1.0, inf, 0.0], [nan, 1.0, 2.0, nan], [nan, nan, nan, nan], [low, low, low, low],
