@@ -351,7 +351,8 @@ int32_t lc_expert_linear(const void* x, int32_t x_dtype, int64_t x_rows, int64_t
  * weights = softmax over all experts (renormalize: over the chosen ones), and every choice's row in the order
  * "by expert, then by token": offsets [experts + 1], positions / chosen / weights [tokens, top_k].  Logits of
  * -inf and NaN are never chosen and carry no weight: chosen and positions are -1 and weights 0 where a token
- * has fewer than top_k others.  experts <= 1024, top_k <= 32.  workspace: lc_route_experts_workspace_bytes. */
+ * has fewer than top_k others.  experts <= 1024, top_k <= 32.  workspace: lc_route_experts_workspace_bytes, 16-byte
+ * aligned, free again when the call's work is done. */
 int64_t lc_route_experts_workspace_bytes(int64_t tokens, int64_t experts);
 int32_t lc_route_experts(const void* logits, int32_t dtype, int64_t tokens, int64_t experts, int64_t ld,
                          int64_t top_k, int32_t renormalize, float* weights, int32_t* chosen, int32_t* offsets,

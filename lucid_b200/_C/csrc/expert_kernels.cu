@@ -1,6 +1,7 @@
 // The kernels around the experts' products: the router (top-k, softmax weights, rows sorted by expert), the
 // row-wise quantizer that also places each token's codes in expert order, and the weighted sum that brings
 // the experts' results back to their tokens.
+#include <algorithm>
 #include <mutex>
 #include <type_traits>
 
@@ -76,10 +77,12 @@ struct RouteParams {
   int32_t* chosen;     // [tokens, top_k]
   int32_t* positions;  // [tokens, top_k]
   int32_t* offsets;    // [experts + 1]
-  int32_t* counts;     // [CTAs, experts], several CTAs only
+  uint16_t* counts;    // [CTAs, count_pitch(experts)], several CTAs only; a CTA has at most 65535 tokens
   int per_cta, run;    // tokens per CTA and per warp
   int vec;             // rows may be read in vectors
 };
+
+__host__ __device__ constexpr int64_t count_pitch(int64_t experts) { return (experts + 7) / 8 * 8; }  // 16-byte loads
 
 // inclusive sum over the block of one int per thread; `tmp` holds 32 ints
 __device__ __forceinline__ int block_scan(int v, int* tmp) {
@@ -252,17 +255,23 @@ __global__ void __launch_bounds__(1024) route_kernel(const RouteParams p) {
 
   // counts of the CTA, and each warp's start inside them
   int* base = s_counts + warps * E;
-  for (int e0 = 0; e0 < E; e0 += blockDim.x) {
+  const int counted = ONE_CTA ? E : static_cast<int>(count_pitch(E));
+  for (int e0 = 0; e0 < counted; e0 += blockDim.x) {
     const int e = e0 + threadIdx.x;
     int sum = 0;
     if (e < E) {
-      for (int w = 0; w < warps; ++w) {
-        const int c = s_counts[w * E + e];
-        s_counts[w * E + e] = sum;
-        sum += c;
+      for (int w = 0; w < warps; w += 8) {  // (a multiple of 8 warps)
+        int c[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = s_counts[(w + i) * E + e];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          s_counts[(w + i) * E + e] = sum;
+          sum += c[i];
+        }
       }
-      if (!ONE_CTA) p.counts[static_cast<int64_t>(blockIdx.x) * E + e] = sum;
     }
+    if (!ONE_CTA && e < counted) p.counts[static_cast<int64_t>(blockIdx.x) * counted + e] = static_cast<uint16_t>(sum);
     if (ONE_CTA) {  // (1024 threads: one round covers all experts)
       const int end = block_scan(sum, s_tmp);
       if (e < E) {
@@ -279,61 +288,121 @@ __global__ void __launch_bounds__(1024) route_kernel(const RouteParams p) {
   }
 }
 
-// second kernel of a large batch: CTA b adds to its tokens' ranks the rows of the experts before and the
-// counts of the CTAs before it.  1024 / (experts rounded up to a power of two, at least 32) groups of threads
-// share the CTAs' counts, one column each.
-__global__ void __launch_bounds__(1024) route_place_kernel(const RouteParams p, int ctas, int64_t tokens_per_cta,
-                                                           int width_log2) {
-  __shared__ int s_sum[1024], s_before[1024];
-  __shared__ int s_tmp[32];
+// Second kernel of a large batch: CTA b adds to its tokens' ranks the rows of the experts before and the counts of the
+// CTAs before it.  Every CTA reads every count (148 x 128: 38 KB), so what costs is latency: 16 bits a count, eight
+// counts a load, and a warp for each 16th or 32nd of the CTAs leave some five loads a thread, which are in flight
+// together with those of the choices.  Before and behind CTA b only whole warps' sums differ, but for the warp that b is
+// in.  512 threads of up to 64 registers share an SM with a CTA of the first kernel (up to 128 experts), so that the next
+// call's begins while this one ends (16384 tokens of 128, 8 of them chosen: 14.8 us a call, with 1024 threads 22.1).  The
+// first kernel for more experts leaves no room in any case, and then more threads read many CTAs' counts sooner (16384
+// tokens of 256: 17.7 us, with 512 threads 19.5; but 128 tokens, four CTAs: 8.3 and 7.6 us).
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
+route_place_kernel(const RouteParams p, int ctas, int64_t tokens_per_cta, int lanes_log2) {
+  constexpr int WARPS = THREADS / 32;
+  constexpr int kSpan = 256;  // experts at a time: 8 a lane
+  __shared__ __align__(16) int s_rows[WARPS][kSpan];
+  __shared__ __align__(16) int s_own[kSpan];
+  __shared__ int s_sum[kRouteMaxExperts], s_before[kRouteMaxExperts], s_tmp[32];
+  const int E = p.experts, pitch = static_cast<int>(count_pitch(E));
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int e = threadIdx.x; e < kRouteMaxExperts; e += THREADS) s_sum[e] = s_before[e] = 0;
   pdl_launch_dependents();
   pdl_wait();
-  const int E = p.experts, width = 1 << width_log2, parts = 1024 >> width_log2;
-  const int e = threadIdx.x & (width - 1), part = threadIdx.x >> width_log2;
-  int before = 0, sum = 0;
-  if (e < E) {
-    const int32_t* c = p.counts + e;
-#pragma unroll 8
-    for (int b = part; b < ctas; b += parts) {
-      const int v = __ldg(c + static_cast<int64_t>(b) * E);
-      if (b < static_cast<int>(blockIdx.x)) before += v;
-      sum += v;
-    }
-  }
-  s_sum[threadIdx.x] = sum;
-  s_before[threadIdx.x] = before;
-  __syncthreads();
-  sum = before = 0;
-  if (static_cast<int>(threadIdx.x) < width)
-    for (int i = 0; i < parts; ++i) {
-      sum += s_sum[(i << width_log2) + e];
-      before += s_before[(i << width_log2) + e];
-    }
-  const int end = block_scan(sum, s_tmp);
-  if (static_cast<int>(threadIdx.x) < E) {
-    s_before[threadIdx.x] = end - sum + before;
-    if (blockIdx.x == 0) {
-      p.offsets[e + 1] = end;
-      if (e == 0) p.offsets[0] = 0;
-    }
-  }
-  __syncthreads();
   const int64_t first = blockIdx.x * tokens_per_cta;
   const int64_t last = first + tokens_per_cta < p.tokens ? first + tokens_per_cta : p.tokens;
-  for (int64_t i = first * p.top_k + threadIdx.x; i < last * p.top_k; i += 1024) {
-    const int at = p.chosen[i];
-    if (at >= 0) p.positions[i] += s_before[at];
+  int64_t item = first * p.top_k + threadIdx.x;
+  const int64_t items_end = last * p.top_k;
+  int at = item < items_end ? p.chosen[item] : -1;
+  int rank = item < items_end ? p.positions[item] : -1;
+
+  const int lanes = 1 << lanes_log2, col = lane & (lanes - 1);
+  const int each = (ctas + WARPS - 1) / WARPS, begin = warp * each, end = min(begin + each, ctas);
+  const int own_warp = static_cast<int>(blockIdx.x) / each;
+  for (int e0 = 0; e0 < pitch; e0 += kSpan) {
+    const int e = e0 + col * 8;
+    int sum[8] = {}, before[8] = {};
+    if (e < pitch) {
+#pragma unroll 5
+      for (int b = begin + (lane >> lanes_log2); b < end; b += 32 >> lanes_log2) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.counts + static_cast<int64_t>(b) * pitch + e));
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        const bool precedes = b < static_cast<int>(blockIdx.x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int c = static_cast<int>(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu);
+          sum[i] += c;
+          before[i] += precedes ? c : 0;
+        }
+      }
+    }
+    for (int o = lanes; o < 32; o <<= 1) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+        before[i] += __shfl_xor_sync(0xffffffffu, before[i], o);
+      }
+    }
+    if (lane < lanes) {
+      int4* row = reinterpret_cast<int4*>(&s_rows[warp][col * 8]);
+      row[0] = make_int4(sum[0], sum[1], sum[2], sum[3]);
+      row[1] = make_int4(sum[4], sum[5], sum[6], sum[7]);
+      if (warp == own_warp) {
+        int4* own = reinterpret_cast<int4*>(&s_own[col * 8]);
+        own[0] = make_int4(before[0], before[1], before[2], before[3]);
+        own[1] = make_int4(before[4], before[5], before[6], before[7]);
+      }
+    }
+    __syncthreads();
+    const int x = threadIdx.x & (kSpan - 1), share = threadIdx.x / kSpan;  // (integer sums: any order)
+    if (e0 + x < E) {
+      int all = 0, some = share == 0 ? s_own[x] : 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int w = share * 8 + i, c = s_rows[w][x];
+        all += c;
+        some += w < own_warp ? c : 0;
+      }
+      atomicAdd(&s_sum[e0 + x], all);
+      atomicAdd(&s_before[e0 + x], some);
+    }
+    __syncthreads();
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.offsets[0] = 0;
+  int preceding = 0;
+  for (int e0 = 0; e0 < E; e0 += THREADS) {
+    const int e = e0 + threadIdx.x, sum = s_sum[e];
+    const int behind = preceding + block_scan(sum, s_tmp);
+    s_before[e] += behind - sum;
+    if (blockIdx.x == 0 && e < E) p.offsets[e + 1] = behind;
+    if (e0 + THREADS < E) {
+      __syncthreads();
+      preceding += s_tmp[WARPS - 1];
+    }
+  }
+  __syncthreads();
+  while (item < items_end) {
+    if (at >= 0) p.positions[item] = rank + s_before[at];
+    item += THREADS;
+    if (item < items_end) {
+      at = p.chosen[item];
+      rank = p.positions[item];
+    }
   }
 }
 
 constexpr int kRouteWarps = 32;
 constexpr int64_t kRouteOneCta = 32;   // tokens (one a warp) that one CTA routes and places in one kernel: 128 tokens of
                                        // 128 experts take 11.5 us that way, 129 on five CTAs and a second kernel 6.9 us
-constexpr int64_t kRouteCtas = 148;    // most CTAs of a larger batch: one for each SM
+constexpr int64_t kRouteCtas = 148;    // CTAs of a larger batch: one for each SM, more behind 9.7 million tokens
 
-int64_t route_per_cta(int64_t tokens) {  // at least one token per warp
+// shared memory of which an SM has no two: where the previous kernel's CTAs leave one by one, two CTAs of the next could
+// meet on one SM while another has none
+constexpr int kRouteOnePerSm = 116 * 1024;
+
+int64_t route_per_cta(int64_t tokens) {  // at least one token per warp, and counts of 16 bits
   const int64_t n = (tokens + kRouteCtas - 1) / kRouteCtas;
-  return n > kRouteWarps ? n : kRouteWarps;
+  return n < kRouteWarps ? kRouteWarps : n < 65535 ? n : 65535;
 }
 
 template <typename T, int EPL>
@@ -346,13 +415,13 @@ cudaError_t launch_route(RouteParams p, cudaStream_t st) {
   constexpr int kLaneBytes = EPL * sizeof(T) < 16 ? EPL * sizeof(T) : 16;
   p.vec = p.experts == 32 * EPL && aligned(p.logits, kLaneBytes) && (p.ld * sizeof(T)) % kLaneBytes == 0;
   std::call_once(flags[dev][one], [dev, one]() {
-    const int bytes = (kRouteWarps + 1) * EPL * 32 * 4;
+    const int bytes = std::max((kRouteWarps + 1) * EPL * 32 * 4, one ? 0 : kRouteOnePerSm);
     results[dev][one] =
         one ? cudaFuncSetAttribute(route_kernel<T, EPL, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)
             : cudaFuncSetAttribute(route_kernel<T, EPL, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   });
   if (results[dev][one] != cudaSuccess) return results[dev][one];
-  const size_t smem = static_cast<size_t>(kRouteWarps + 1) * p.experts * 4;
+  const size_t smem = std::max<size_t>(static_cast<size_t>(kRouteWarps + 1) * p.experts * 4, one ? 0 : kRouteOnePerSm);
   const int64_t per_cta = one ? p.tokens : route_per_cta(p.tokens);
   p.per_cta = static_cast<int>(per_cta);
   p.run = static_cast<int>((per_cta + kRouteWarps - 1) / kRouteWarps);
@@ -360,9 +429,11 @@ cudaError_t launch_route(RouteParams p, cudaStream_t st) {
   const int ctas = static_cast<int>((p.tokens + per_cta - 1) / per_cta);
   cudaError_t err = launch_overlapped(route_kernel<T, EPL, false>, dim3(ctas), dim3(1024), smem, st, p);
   if (err != cudaSuccess) return err;
-  int width_log2 = 5;
-  while ((1 << width_log2) < p.experts) ++width_log2;
-  return launch_overlapped(route_place_kernel, dim3(ctas), dim3(1024), 0, st, p, ctas, per_cta, width_log2);
+  int lanes_log2 = 0;
+  while (lanes_log2 < 5 && (8 << lanes_log2) < p.experts) ++lanes_log2;
+  if (EPL > 4 && ctas > 32)
+    return launch_overlapped(route_place_kernel<1024>, dim3(ctas), dim3(1024), 0, st, p, ctas, per_cta, lanes_log2);
+  return launch_overlapped(route_place_kernel<512>, dim3(ctas), dim3(512), 0, st, p, ctas, per_cta, lanes_log2);
 }
 
 template <typename T>
@@ -782,7 +853,7 @@ using namespace lc;
 extern "C" int64_t lc_route_experts_workspace_bytes(int64_t tokens, int64_t experts) {
   if (tokens <= kRouteOneCta || experts <= 0) return 0;
   const int64_t per_cta = route_per_cta(tokens);
-  return (tokens + per_cta - 1) / per_cta * experts * 4;
+  return (tokens + per_cta - 1) / per_cta * count_pitch(experts) * 2;
 }
 
 extern "C" int32_t lc_route_experts(const void* logits, int32_t dtype, int64_t tokens, int64_t experts, int64_t ld,
@@ -804,7 +875,7 @@ extern "C" int32_t lc_route_experts(const void* logits, int32_t dtype, int64_t t
   }
   if (!logits || !weights || !chosen || !positions) return fail(LC_ERR_INVALID_ARG, "route_experts: null pointer");
   const int64_t need = lc_route_experts_workspace_bytes(tokens, experts);
-  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 4)))
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(LC_ERR_WORKSPACE, "route_experts: workspace of %lld bytes required", (long long)need);
   RouteParams p = {};
   p.logits = logits;
@@ -817,7 +888,7 @@ extern "C" int32_t lc_route_experts(const void* logits, int32_t dtype, int64_t t
   p.chosen = chosen;
   p.positions = positions;
   p.offsets = offsets;
-  p.counts = static_cast<int32_t*>(workspace);
+  p.counts = static_cast<uint16_t*>(workspace);
   cudaStream_t st = as_stream(stream);
   return finish_launch("route_experts", dtype == LC_F32    ? dispatch_route<float>(p, st)
                                         : dtype == LC_BF16 ? dispatch_route<__nv_bfloat16>(p, st)

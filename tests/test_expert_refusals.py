@@ -137,6 +137,7 @@ def test_c_entry_points_refuse_before_they_launch():
     assert L.lc_route_experts(p, capi.LC_F32, 4, 8, 8, 9, 1, p, p, p, p, None, 0, None) == invalid
     assert L.lc_route_experts(p, capi.LC_F32, 4, 2000, 2000, 2, 1, p, p, p, p, None, 0, None) == unsupported
     assert L.lc_route_experts(p, capi.LC_F32, 4096, 8, 8, 2, 1, p, p, p, p, None, 0, None) == capi.LC_ERR_WORKSPACE
+    assert L.lc_route_experts(p, capi.LC_F32, 4096, 8, 8, 2, 1, p, p, p, p, p + 8, 4096, None) == capi.LC_ERR_WORKSPACE
     assert L.lc_combine_experts(p, capi.LC_F32, 4, 8, 8, p, p, 2, 0, None, 0, p, 8, None) == invalid
     assert L.lc_combine_experts(p, capi.LC_U8, 4, 8, 8, p, p, 2, 2, None, 0, p, 8, None) == unsupported
     assert L.lc_expert_linear(p, capi.LC_F32, 4, 32, None, 1, None, 1, 4, p, 32, 0, 16, 32, p, None, 0, None, 0, p,

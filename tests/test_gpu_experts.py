@@ -334,6 +334,21 @@ def test_route_equal_logits(F, experts, top_k):
     np.testing.assert_allclose(r.weights.cpu().numpy(), weights, rtol=48 * 2.0 ** -23)
 
 
+@pytest.mark.parametrize("tokens,experts,top_k", [(5000, 600, 4), (6001, 1024, 2), (20000, 255, 8), (3333, 12, 12), (9_800_000, 3, 1)])
+def test_route_many_tokens(F, tokens, experts, top_k):
+    # the order "by expert, then by token" is the stable sort of the choices, which a sort of integers gives exactly
+    logits = torch.randn(tokens, experts, generator=generator(tokens), device="cuda")
+    r = F.route_experts(logits, top_k)
+    assert torch.equal(r.experts.long(), torch.sort(logits, dim=1, descending=True, stable=True)[1][:, :top_k])
+    flat = r.experts.reshape(-1).long()
+    order = torch.sort(flat, stable=True)[1]
+    positions = torch.empty_like(order)
+    positions[order] = torch.arange(order.numel(), device="cuda")
+    assert torch.equal(r.positions.reshape(-1).long(), positions)
+    counts = torch.bincount(flat, minlength=experts)
+    assert torch.equal(r.offsets.long(), torch.cat([counts.new_zeros(1), counts.cumsum(0)]))
+
+
 def test_route_special_logits(F):
     inf, nan, low = math.inf, math.nan, torch.finfo(torch.float32).min
     logits = torch.tensor([[inf, 1.0, inf, 0.0], [nan, 1.0, 2.0, nan], [nan, nan, nan, nan], [low, low, low, low],
