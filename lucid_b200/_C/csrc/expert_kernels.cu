@@ -135,7 +135,9 @@ template <typename T, int EPL, bool ONE_CTA>
 __global__ void __launch_bounds__(1024) route_kernel(const RouteParams p) {
   extern __shared__ int s_counts[];  // [warps][experts]; one CTA: then [experts] bases
   __shared__ int s_tmp[32];
+  __shared__ uint2 s_pick[32][kRouteMaxTopK];  // a token's choices: value, expert
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t below = (1u << lane) - 1u;
   const int E = p.experts, K = p.top_k;
   int* mine = s_counts + warp * E;
   for (int i = threadIdx.x; i < warps * E; i += blockDim.x) s_counts[i] = 0;
@@ -194,17 +196,15 @@ __global__ void __launch_bounds__(1024) route_kernel(const RouteParams p) {
             if (swap) from[l] ^= bits << 2 * i | bits << 2 * (i + 1);
           }
       }
-      for (int j = 0; j < K && best; ++j) {
+      int j = 0;
+      for (; j < K && best; ++j) {
         const bool second = LISTS > 1 && key[0] != best;
         const uint32_t head = second ? key[EPL - LEN] : key[0];
-        const int at = lane * EPL + (second ? LEN + static_cast<int>(from[LISTS - 1] & 3u) : static_cast<int>(from[0] & 3u));
-        const int winner = __ffs(__ballot_sync(0xffffffffu, head == best)) - 1;
-        const int e = __shfl_sync(0xffffffffu, at, winner);
-        if (lane == j) {
-          my_key = best;
-          my_e = e;
-        }
-        if (lane == winner) {
+        const bool equal = head == best;
+        const uint32_t who = __ballot_sync(0xffffffffu, equal);
+        if (equal && !(who & below)) {  // the lowest lane of several
+          const int at = second ? LEN + static_cast<int>(from[LISTS - 1] & 3u) : static_cast<int>(from[0] & 3u);
+          s_pick[warp][j] = make_uint2(best, lane * EPL + at);
 #pragma unroll
           for (int l = 0; l < LISTS; ++l) {
             if (second != (l == 1)) continue;
@@ -214,6 +214,12 @@ __global__ void __launch_bounds__(1024) route_kernel(const RouteParams p) {
           }
         }
         best = __reduce_max_sync(0xffffffffu, LISTS > 1 ? max(key[0], key[EPL - LEN]) : key[0]);
+      }
+      __syncwarp();
+      if (lane < j) {
+        const uint2 pick = s_pick[warp][lane];
+        my_key = pick.x;
+        my_e = static_cast<int>(pick.y);
       }
     } else {
       for (int j = 0; j < K && best; ++j) {
