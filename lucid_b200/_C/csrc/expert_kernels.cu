@@ -49,8 +49,9 @@ struct Vec16 {
 // one warp-wide integer maximum (order-preserving bits of the value) and a vote: of several lanes with the largest
 // value the lowest has the lowest expert, and that lane moves on to its next one.  Up to eight values a
 // lane are sorted first, in lists of up to four, so that moving on is a shift (16384 tokens of 256 experts, 8 of them
-// chosen: 21.3 us, 24.1 with a search for the lane's next value); more are searched.  The kernel is bound by the instructions of a token
-// (16384 tokens of 128 experts, 8 of them chosen: 498), 16.8 us together with the second kernel's latency.
+// chosen: 24.1 -> 21.3 us with nothing else changed, now 17.1); more are searched.  The kernel is bound by the instructions of a token
+// (16384 tokens of 128 experts, 8 of them chosen: 480, three quarters of the issue slots), 13.8 us together with the
+// second kernel's latency.  The winning lane leaves its choice in shared memory: broadcast by shuffle it was 14.8 us.
 // A warp walks a contiguous run of tokens and counts its choices per expert in shared memory; a choice's
 // count is its rank inside the run.  Small batches (one CTA) finish in the same kernel; otherwise each CTA
 // leaves its counts and its ranks, and the second kernel adds what precedes them.  Every sum is an integer
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(1024) route_kernel(const RouteParams p) {
 // counts a load, and a warp for each 16th or 32nd of the CTAs leave some five loads a thread, which are in flight
 // together with those of the choices.  Before and behind CTA b only whole warps' sums differ, but for the warp that b is
 // in.  512 threads of up to 64 registers share an SM with a CTA of the first kernel (up to 128 experts), so that the next
-// call's begins while this one ends (16384 tokens of 128, 8 of them chosen: 14.8 us a call, with 1024 threads 22.1).  The
+// call's begins while this one ends (16384 tokens of 128, 8 of them chosen: 22.1 us a call with 1024 threads, then 14.8).  The
 // first kernel for more experts leaves no room in any case, and then more threads read many CTAs' counts sooner (16384
 // tokens of 256: 17.7 us, with 512 threads 19.5; but 128 tokens, four CTAs: 8.3 and 7.6 us).
 template <int THREADS>
@@ -399,7 +400,7 @@ route_place_kernel(const RouteParams p, int ctas, int64_t tokens_per_cta, int la
 
 constexpr int kRouteWarps = 32;
 constexpr int64_t kRouteOneCta = 32;   // tokens (one a warp) that one CTA routes and places in one kernel: 128 tokens of
-                                       // 128 experts take 11.5 us that way, 129 on five CTAs and a second kernel 6.9 us
+                                       // 128 experts take 11.5 us that way, on four CTAs and a second kernel 6.2 us
 constexpr int64_t kRouteCtas = 148;    // CTAs of a larger batch: one for each SM, more behind 9.7 million tokens
 
 // shared memory of which an SM has no two: where the previous kernel's CTAs leave one by one, two CTAs of the next could
